@@ -172,6 +172,38 @@ typedef struct {
   int fz;
 } DmlExpandReduceArgs;
 
+// Pointwise functions behind a norm or a product (csrc/kernels/activation.h), and tensor types.
+enum { DML_ACT_NONE, DML_ACT_RELU, DML_ACT_SILU, DML_ACT_GELU, DML_ACT_GELU_TANH, DML_ACT_COUNT };
+enum { DML_BF16, DML_F16, DML_F32 };
+
+// Group norm + affine + activation, channels last (csrc/kernels/group_norm.hip): sample n, pixel p
+// at x + n*xn + p*ldx (elements), the C channels contiguous.
+typedef struct {
+  const void* x;
+  void* y;              // same type; may be x itself
+  const float* weight;  // fp32 [C] or null (1)
+  const float* bias;    // fp32 [C] or null (0)
+  int64_t xn, yn, ldx, ldy;
+  int N, HW, C, G;
+  int dtype, act;
+  float eps;
+} DmlGroupNormArgs;
+
+// Matrix product with a fused epilogue (csrc/kernels/product.hip): y = act(x . W_e^T + b_e) + res, or
+// act(x . W_e^T + b_e + res) with act_last, W_e the weight of the group that the row belongs to.
+typedef struct {
+  const void* x;      // [M][ldx], K used
+  const void* w;      // [E][N][ldw], K used, group pitch w_group; type of x
+  const float* bias;  // fp32 [E][N], group pitch bias_group, or null
+  const void* res;    // [M][ldr], type of y, or null; may be y itself
+  void* y;            // [M][ldy], N written: type of x, or fp32 with out_f32
+  const void* ends;   // device: group e's rows end before ends[e] (int32, int64 with ends64); null: one group
+  int64_t ldx, ldw, w_group, bias_group, ldr, ldy;
+  int M, N, K, E;
+  int dtype, out_f32, act, act_last, ends64;
+  int fill;           // 1: rows behind the last group are set to 0; 0: left as they are
+} DmlProductArgs;
+
 // ---- single-op launches (used by tests and by the plan executor) ----
 int dml_stem_resnet(const DmlStemArgs* a, hipStream_t s);
 int dml_stem_inception(const DmlIncStemArgs* a, hipStream_t s);
@@ -233,6 +265,8 @@ int dml_softmax_top5(const float* logits, int B, int classes, int ld, float* pro
 // slice 0 before the softmax.
 int dml_softmax_top5_split(float* logits, int B, int classes, int ld, int nsplit, int split_ld,
                            float* probs_out, int* top_idx, float* top_p, hipStream_t s);
+int dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s);
+int dml_product(const DmlProductArgs* a, hipStream_t s);
 int dml_preprocess(const DmlPreprocArgs* a, hipStream_t s);
 int dml_index_fetch(const int* host, int* dev, int n, hipStream_t s);  // pinned host table -> device
 // packed full-resolution RGB images -> arena slots, nearest resize (misc.hip resize_nearest_kernel)

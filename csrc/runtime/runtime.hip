@@ -45,7 +45,8 @@ extern "C" int dml_device_info(int* cus, int* arch_major, int* arch_minor) {
 extern "C" int dml_abi_sizes(int* out, int n) {
   const int sz[] = {(int)sizeof(DmlConvArgs), (int)sizeof(DmlPoolArgs), (int)sizeof(DmlConvGroupArgs),
                     (int)sizeof(DmlPreprocArgs), (int)sizeof(DmlStemArgs), (int)sizeof(DmlIncStemArgs),
-                    (int)sizeof(DmlConvPoolArgs), (int)sizeof(DmlExpandReduceArgs)};
+                    (int)sizeof(DmlConvPoolArgs), (int)sizeof(DmlExpandReduceArgs),
+                    (int)sizeof(DmlGroupNormArgs), (int)sizeof(DmlProductArgs)};
   const int m = (int)(sizeof(sz) / sizeof(sz[0]));
   for (int i = 0; i < n && i < m; ++i) out[i] = sz[i];
   return m;

@@ -32,6 +32,8 @@ SOURCES = [
     CSRC / "kernels" / "stem_fused.hip",
     CSRC / "kernels" / "conv_pool.hip",
     CSRC / "kernels" / "expand_reduce_chain.hip",
+    CSRC / "kernels" / "group_norm.hip",
+    CSRC / "kernels" / "product.hip",
     CSRC / "runtime" / "runtime.hip",
 ]
 HEADERS = [CSRC / "include" / "dml.h"] + sorted((CSRC / "kernels").glob("*.h"))  # every header the stamp covers

@@ -98,7 +98,30 @@ class ExpandReduceArgs(C.Structure):
     ]
 
 
+class GroupNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("y", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("xn", C.c_int64), ("yn", C.c_int64), ("ldx", C.c_int64), ("ldy", C.c_int64),
+        ("N", C.c_int), ("HW", C.c_int), ("C", C.c_int), ("G", C.c_int),
+        ("dtype", C.c_int), ("act", C.c_int), ("eps", C.c_float),
+    ]
+
+
+class ProductArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("res", C.c_void_p), ("y", C.c_void_p),
+        ("ends", C.c_void_p),
+        ("ldx", C.c_int64), ("ldw", C.c_int64), ("w_group", C.c_int64), ("bias_group", C.c_int64),
+        ("ldr", C.c_int64), ("ldy", C.c_int64),
+        ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("E", C.c_int),
+        ("dtype", C.c_int), ("out_f32", C.c_int), ("act", C.c_int), ("act_last", C.c_int), ("ends64", C.c_int),
+        ("fill", C.c_int),
+    ]
+
+
 _SIGS = {
+    "dml_group_norm": (C.c_int, [C.POINTER(GroupNormArgs), C.c_void_p]),
+    "dml_product": (C.c_int, [C.POINTER(ProductArgs), C.c_void_p]),
     "dml_expand_reduce": (C.c_int, [C.POINTER(ExpandReduceArgs), C.c_void_p]),
     "dml_chain_supported": (C.c_int, [C.POINTER(ExpandReduceArgs)]),
     "dml_plan_add_expand_reduce": (C.c_int, [C.c_void_p, C.POINTER(ExpandReduceArgs)]),
@@ -182,7 +205,7 @@ class NativeError(RuntimeError):
 
 
 ABI_STRUCTS = ("ConvArgs", "PoolArgs", "ConvGroupArgs", "PreprocArgs", "StemArgs", "IncStemArgs", "ConvPoolArgs",
-               "ExpandReduceArgs")
+               "ExpandReduceArgs", "GroupNormArgs", "ProductArgs")
 
 
 def _check_abi(L) -> None:

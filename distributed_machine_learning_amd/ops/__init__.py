@@ -13,9 +13,11 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native as N
+from .layers import grouped_linear, group_norm, linear
 
 __all__ = ["conv2d_nhwc", "conv_group", "pool3x3", "global_avgpool", "softmax_top5", "preprocess", "pack_weight",
-           "resnet_stem", "inception_stem", "conv3x3_pool", "expand_reduce"]
+           "resnet_stem", "inception_stem", "conv3x3_pool", "expand_reduce", "group_norm", "linear",
+           "grouped_linear"]
 
 
 def _r(x, m):

@@ -1,0 +1,247 @@
+"""Group norm and the fused matrix products (csrc/kernels/group_norm.hip, product.hip).
+
+Channels last like every op here: the last dimension is contiguous, the leading ones may be a slice of a
+wider (concat) buffer. Forward only, on the tensors' device and its current stream; a call allocates its
+output and nothing that outlives it, so it can be captured into a graph. Wrong arguments raise TypeError
+or ValueError before anything is launched, a failure of the library raises ``NativeError``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _native as N
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # DML_ACT_*
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # DML_BF16, DML_F16, DML_F32
+_INT = 2 ** 31 - 1
+
+
+def _act(act: str) -> int:
+    try:
+        return ACTIVATIONS[act]
+    except (KeyError, TypeError):
+        raise ValueError(f"act is one of {', '.join(ACTIVATIONS)}: got {act!r}") from None
+
+
+def _pitch(t: torch.Tensor, first: int, what: str) -> Tuple[int, int]:
+    """(rows, elements from one row to the next) of dimensions first .. -2 of t seen as rows of its last one."""
+    shape, stride = t.shape, t.stride()
+    if shape[-1] > 1 and stride[-1] != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous, got strides {stride}")
+    rows, pitch = 1, None
+    for d in range(t.dim() - 2, first - 1, -1):
+        n = shape[d]
+        if n != 1:
+            if pitch is None:
+                pitch = stride[d]
+            elif stride[d] != pitch * rows and rows:
+                raise ValueError(f"{what}: dimensions {first} to {t.dim() - 2} must step as one, got shape "
+                                 f"{tuple(shape)} with strides {stride}")
+            rows *= n
+    return rows, shape[-1] if pitch is None else pitch
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte and the one behind the last of what t may touch."""
+    p = t.data_ptr()
+    return p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _apart(out: torch.Tensor, t: Optional[torch.Tensor], what: str, same: bool = False) -> None:
+    """out must share no memory with t: unless (same) it is t itself, or they are other columns of one buffer."""
+    if t is None or not out.numel() or not t.numel():
+        return
+    a, b = _span(out)
+    c, d = _span(t)
+    if b <= c or d <= a:
+        return
+    if same and a == c and out.shape == t.shape and out.stride() == t.stride() and out.dtype == t.dtype:
+        return
+    steps = [s for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1]
+    if steps and out.element_size() == t.element_size() and out.stride() == t.stride() and out.shape[:-1] == t.shape[:-1]:
+        pitch = min(steps) * out.element_size()
+        gap = (c - a) % pitch  # t's columns begin here in out's rows
+        if abs(c - a) < pitch and gap >= out.shape[-1] * out.element_size() \
+                and gap + t.shape[-1] * t.element_size() <= pitch:
+            return
+    raise ValueError(f"out overlaps {what}")
+
+
+def _vector(v: Optional[torch.Tensor], shape: Tuple[int, ...], dtype: torch.dtype, what: str) -> None:
+    if v is None:
+        return
+    if tuple(v.shape) != shape:
+        raise ValueError(f"{what}: expected shape {shape}, got {tuple(v.shape)}")
+    if v.dtype is not torch.float32 and v.dtype is not dtype:
+        raise TypeError(f"{what}: expected float32 or {dtype}, got {v.dtype}")
+
+
+def _ready(*tensors: Optional[torch.Tensor]) -> None:
+    """All on one HIP device, and none that autograd would expect a gradient for."""
+    dev = tensors[0].device
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None:
+            if t.device != dev:
+                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+            if grad and t.requires_grad:
+                raise ValueError("this operator has no backward: call it under torch.no_grad()")
+    if dev.type != "cuda":
+        raise ValueError(f"expected tensors on a HIP device, got {dev}")
+
+
+def _launch(fn, args, device: torch.device, what: str) -> None:
+    if device.index == torch.cuda.current_device():
+        N.check(fn(C.byref(args), N.stream_ptr()), what)
+    else:
+        with torch.cuda.device(device):
+            N.check(fn(C.byref(args), N.stream_ptr()), what)
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5, act: str = "none",
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Group norm, affine map and activation of channels-last features.
+
+    x: [N, ..., C] bf16, fp16 or fp32; the dimensions between step as one (NHWC maps, [N, L, C] tokens, a
+    channel slice of a concat buffer), any pitch between samples. Mean and variance (biased) go over all
+    positions and the C / groups channels of a group, in fp32. weight, bias: [C], fp32 or x's type, or None.
+    act: "none", "relu", "silu", "gelu" or "gelu_tanh". out: x's shape and type; may be x itself.
+    """
+    code = _act(act)
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"x: expected bfloat16, float16 or float32, got {x.dtype}")
+    if x.dim() < 2:
+        raise ValueError(f"x: expected [N, ..., C], got shape {tuple(x.shape)}")
+    n, c = x.shape[0], x.shape[-1]
+    if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or c < 1 or c % groups:
+        raise ValueError(f"groups must divide the {c} channels, got {groups!r}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    _vector(weight, (c,), x.dtype, "weight")
+    _vector(bias, (c,), x.dtype, "bias")
+    rows, ldx = _pitch(x, 1, "x")
+    if out is None:
+        ldy = c
+    else:
+        if out.shape != x.shape or out.dtype is not x.dtype:
+            raise ValueError(f"out: expected {x.dtype} of shape {tuple(x.shape)}, got {out.dtype} of {tuple(out.shape)}")
+        _, ldy = _pitch(out, 1, "out")
+        if (rows > 1 and ldy < c) or (n > 1 and out.stride(0) < c):
+            raise ValueError("out: its positions overlap each other")
+        _apart(out, x, "x", same=True)
+        _apart(out, weight, "weight")
+        _apart(out, bias, "bias")
+    if n > _INT or rows > _INT or n * groups > _INT:
+        raise ValueError("x: over 2^31 - 1 samples, positions or groups")
+    _ready(x, weight, bias, out)
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if not out.numel():
+        return out
+    if weight is not None:
+        weight = weight.float().contiguous()
+    if bias is not None:
+        bias = bias.float().contiguous()
+    a = N.GroupNormArgs(x.data_ptr(), out.data_ptr(), weight.data_ptr() if weight is not None else None,
+                        bias.data_ptr() if bias is not None else None, x.stride(0), out.stride(0),
+                        ldx, ldy, n, rows, c, groups, _DTYPES[x.dtype], code, eps)
+    _launch(N.lib().dml_group_norm, a, x.device, "dml_group_norm")
+    return out
+
+
+def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, what):
+    code = _act(act)
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
+        raise TypeError(f"x: expected bfloat16 or float16, got {x.dtype}")
+    if weight.dtype is not x.dtype:
+        raise TypeError(f"weight: expected {x.dtype} like x, got {weight.dtype}")
+    wdim = 2 if ends is None else 3
+    if weight.dim() != wdim or x.dim() < 1 or weight.shape[-1] != x.shape[-1]:
+        raise ValueError(f"{what}: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    n, k = weight.shape[-2], weight.shape[-1]
+    e = 1 if ends is None else weight.shape[0]
+    shape = (*x.shape[:-1], n)
+    to = out.dtype if out is not None else out_dtype if out_dtype is not None else x.dtype
+    if to is not x.dtype and to is not torch.float32:
+        raise TypeError(f"out: expected {x.dtype} or float32, got {to}")
+    if out_dtype is not None and out_dtype is not to:
+        raise TypeError(f"out is {to}, out_dtype {out_dtype}")
+    _vector(bias, (n,) if ends is None else (e, n), x.dtype, "bias")
+    m, ldx = _pitch(x, 0, "x")
+    _, ldw = _pitch(weight, wdim - 2, "weight")
+    if residual is not None:
+        if tuple(residual.shape) != shape or residual.dtype is not to:
+            raise ValueError(f"residual: expected {to} of shape {shape}, got {residual.dtype} of "
+                             f"{tuple(residual.shape)}")
+        ldr = _pitch(residual, 0, "residual")[1]
+    if out is None:
+        ldy = n
+    else:
+        if tuple(out.shape) != shape:
+            raise ValueError(f"out: expected shape {shape}, got {tuple(out.shape)}")
+        ldy = _pitch(out, 0, "out")[1]
+        if m > 1 and ldy < n:
+            raise ValueError("out: its rows overlap each other")
+        _apart(out, x, "x")
+        _apart(out, weight, "weight")
+        _apart(out, bias, "bias")
+        _apart(out, ends, "ends")
+        _apart(out, residual, "residual", same=True)
+    if max(m, n, k, e) > _INT - 512:
+        raise ValueError(f"{what}: a dimension over 2^31 - 513")
+    _ready(x, weight, ends, bias, residual, out)
+    fill = 0
+    if out is None:
+        out = torch.empty(shape, device=x.device, dtype=to)
+        fill = int(ends is not None)
+    if not out.numel():
+        return out
+    if e == 0:
+        return out.zero_() if fill else out
+    if bias is not None:
+        bias = bias.float().contiguous()
+    a = N.ProductArgs(x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
+                      residual.data_ptr() if residual is not None else None, out.data_ptr(),
+                      ends.data_ptr() if ends is not None else None, ldx, ldw,
+                      weight.stride(0) if wdim == 3 else 0, n, ldr if residual is not None else 0, ldy,
+                      m, n, k, e, _DTYPES[x.dtype], int(to is torch.float32), code, int(bool(act_last)),
+                      int(ends is not None and ends.dtype is torch.int64), fill)
+    _launch(N.lib().dml_product, a, x.device, what)
+    return out
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
+           residual: Optional[torch.Tensor] = None, act_last: bool = False, out: Optional[torch.Tensor] = None,
+           out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x . weight^T + bias) + residual, or with act_last act(x . weight^T + bias + residual).
+
+    x: [..., K] bf16 or fp16, the leading dimensions stepping as one; weight: [N, K] of x's type (rows may be
+    padded); any sizes, a product over K = 0 is 0. bias: [N], fp32 or x's type. residual: [..., N] of the output's
+    type (an expanded one is read where it lies). Output [..., N] of x's type, or fp32 with out_dtype; out may be
+    the residual itself, or a column slice of a wider buffer. Sums in fp32, one rounding at the end.
+    """
+    return _product(x, weight, None, bias, act, residual, act_last, out, out_dtype, "linear")
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   act: str = "none", residual: Optional[torch.Tensor] = None, act_last: bool = False,
+                   out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """linear() with a weight per group of rows: rows ends[e-1] (0 for the first group) to ends[e] - 1 of x go
+    through weight[e] and bias[e].
+
+    x: [T, K] with its rows in the groups' order; weight: [E, N, K]; bias: [E, N]; ends: [E] int32 or int64 on the
+    device, ascending, at most T (the counts' cumulative sum). Groups may be empty. The ends stay on the device:
+    the host does not wait for them, and a captured call follows them from replay to replay. Out-of-order or
+    out-of-range ends are clamped to an ascending sequence in [0, T]. Rows behind the last group stay as they are
+    in out; without out they are 0.
+    """
+    if ends.dtype is not torch.int32 and ends.dtype is not torch.int64:
+        raise TypeError(f"ends: expected int32 or int64, got {ends.dtype}")
+    if weight.dim() != 3 or x.dim() != 2 or tuple(ends.shape) != (weight.shape[0],) or not ends.is_contiguous():
+        raise ValueError(f"grouped_linear: expected x [T, K], weight [E, N, K] and contiguous ends [E], got "
+                         f"{tuple(x.shape)}, {tuple(weight.shape)} and {tuple(ends.shape)}")
+    return _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, "grouped_linear")

@@ -1,0 +1,113 @@
+"""Arguments that ops.group_norm, ops.linear and ops.grouped_linear refuse, before anything reaches a device."""
+import pytest
+import torch
+
+from distributed_machine_learning_amd import _native as N
+from distributed_machine_learning_amd import ops
+
+BF = torch.bfloat16
+
+
+def _t(*shape, dtype=BF):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def _norm(x=None, groups=4, **kw):
+    return ops.group_norm(_t(2, 3, 3, 16) if x is None else x, groups, **kw)
+
+
+BUF = torch.zeros(4, 64, dtype=BF)
+
+
+@pytest.mark.parametrize("error, match, call", [
+    (ValueError, "act is one of", lambda: _norm(act="tanh")),
+    (ValueError, "act is one of", lambda: _norm(act=None)),
+    (TypeError, "x: expected", lambda: _norm(_t(2, 3, 16, dtype=torch.float64))),
+    (ValueError, "expected \\[N", lambda: _norm(_t(16))),
+    (ValueError, "groups must divide", lambda: _norm(groups=5)),
+    (ValueError, "groups must divide", lambda: _norm(groups=0)),
+    (ValueError, "groups must divide", lambda: _norm(groups=True)),
+    (ValueError, "groups must divide", lambda: _norm(_t(2, 3, 0))),
+    (ValueError, "eps", lambda: _norm(eps=-1e-5)),
+    (ValueError, "eps", lambda: _norm(eps=float("nan"))),
+    (ValueError, "weight: expected shape", lambda: _norm(weight=_t(8))),
+    (TypeError, "bias: expected", lambda: _norm(bias=_t(16, dtype=torch.float16))),
+    (ValueError, "last dimension", lambda: _norm(_t(2, 16, 9).transpose(1, 2))),
+    (ValueError, "step as one", lambda: _norm(_t(2, 6, 3, 16)[:, ::2, :2])),
+    (ValueError, "out: expected", lambda: _norm(out=_t(2, 9, 16))),
+    (ValueError, "out: expected", lambda: _norm(out=_t(2, 3, 3, 16, dtype=torch.float32))),
+    (ValueError, "overlap each other", lambda: _norm(_t(2, 9, 16), out=_t(2, 1, 16).expand(2, 9, 16))),
+    (ValueError, "out overlaps x", lambda: _norm(BUF[:, :16], out=BUF[:, 8:24])),
+    (ValueError, "HIP device", lambda: _norm()),
+    (ValueError, "HIP device", lambda: _norm(BUF[:, :16], out=BUF[:, 16:32])),  # other columns: no overlap
+    (ValueError, "HIP device", lambda: _norm(BUF[:, :16], out=BUF[:, :16])),    # in place
+    (ValueError, "no backward", lambda: _norm(weight=torch.ones(16, requires_grad=True))),
+])
+def test_group_norm_refuses(error, match, call):
+    with pytest.raises(error, match=match):
+        call()
+
+
+def _lin(x=None, w=None, **kw):
+    return ops.linear(_t(4, 8) if x is None else x, _t(6, 8) if w is None else w, **kw)
+
+
+@pytest.mark.parametrize("error, match, call", [
+    (ValueError, "act is one of", lambda: _lin(act="swish")),
+    (TypeError, "x: expected", lambda: _lin(_t(4, 8, dtype=torch.float32))),
+    (TypeError, "weight: expected", lambda: _lin(w=_t(6, 8, dtype=torch.float16))),
+    (ValueError, "does not fit", lambda: _lin(w=_t(6, 7))),
+    (ValueError, "does not fit", lambda: _lin(w=_t(2, 6, 8))),
+    (ValueError, "does not fit", lambda: _lin(torch.tensor(1.0, dtype=BF))),
+    (ValueError, "last dimension", lambda: _lin(w=_t(8, 6).t())),
+    (ValueError, "last dimension", lambda: _lin(_t(8, 4).t())),
+    (ValueError, "step as one", lambda: _lin(_t(4, 5, 8)[:, :3])),
+    (ValueError, "bias: expected shape", lambda: _lin(bias=_t(5))),
+    (TypeError, "bias: expected", lambda: _lin(bias=_t(6, dtype=torch.float16))),
+    (TypeError, "out: expected", lambda: _lin(out_dtype=torch.float16)),
+    (TypeError, "out is", lambda: _lin(out=_t(4, 6), out_dtype=torch.float32)),
+    (ValueError, "out: expected shape", lambda: _lin(out=_t(4, 5))),
+    (ValueError, "rows overlap", lambda: _lin(out=_t(1, 6).expand(4, 6))),
+    (ValueError, "residual: expected", lambda: _lin(residual=_t(4, 6, dtype=torch.float32))),
+    (ValueError, "residual: expected", lambda: _lin(residual=_t(6))),
+    (ValueError, "out overlaps x", lambda: _lin(BUF[:, :8], out=BUF[:, 2:8])),
+    (ValueError, "out overlaps weight", lambda: _lin(w=BUF[:, :8], out=BUF[:, 4:8])),
+    (ValueError, "out overlaps residual", lambda: _lin(residual=BUF[:, 1:7], out=BUF[:, :6])),
+    (ValueError, "no backward", lambda: _lin(w=_t(6, 8).requires_grad_())),
+    (ValueError, "HIP device", lambda: _lin(residual=BUF[:, :6], out=BUF[:, :6])),
+    (ValueError, "HIP device", lambda: _lin(BUF[:, :8], out=BUF[:, 8:14])),
+    (ValueError, "different devices", lambda: _lin(bias=torch.zeros(6, device="meta"))),
+])
+def test_linear_refuses(error, match, call):
+    with pytest.raises(error, match=match):
+        call()
+
+
+def _grp(x=None, w=None, ends=None, **kw):
+    ends = torch.tensor([1, 4], dtype=torch.int32) if ends is None else ends
+    return ops.grouped_linear(_t(4, 8) if x is None else x, _t(2, 6, 8) if w is None else w, ends, **kw)
+
+
+@pytest.mark.parametrize("error, match, call", [
+    (TypeError, "ends: expected", lambda: _grp(ends=torch.tensor([1.0, 4.0]))),
+    (ValueError, "contiguous ends", lambda: _grp(ends=torch.tensor([1, 2, 4]))),
+    (ValueError, "contiguous ends", lambda: _grp(ends=torch.tensor([1, 0, 4, 0])[::2])),
+    (ValueError, "expected x \\[T, K\\]", lambda: _grp(_t(2, 2, 8))),
+    (ValueError, "expected x \\[T, K\\]", lambda: _grp(w=_t(6, 8))),
+    (ValueError, "does not fit", lambda: _grp(w=_t(2, 6, 7))),
+    (ValueError, "bias: expected shape", lambda: _grp(bias=_t(6))),
+    (ValueError, "last dimension", lambda: _grp(w=_t(2, 8, 6).transpose(1, 2))),
+    (ValueError, "residual: expected", lambda: _grp(residual=_t(3, 6))),
+    (ValueError, "out overlaps ends", lambda: (lambda e: _grp(ends=e, out=e.view(BF).as_strided((4, 6), (6, 1))))(
+        torch.zeros(32, dtype=torch.int32)[:2].contiguous())),
+    (ValueError, "HIP device", lambda: _grp()),
+])
+def test_grouped_linear_refuses(error, match, call):
+    with pytest.raises(error, match=match):
+        call()
+
+
+def test_argument_structs_match_the_library():
+    """lib() compares the struct sizes; the new ones are among those compared."""
+    assert {"GroupNormArgs", "ProductArgs"} <= set(N.ABI_STRUCTS)
+    N.lib()

@@ -1,0 +1,511 @@
+"""ops.group_norm, ops.linear and ops.grouped_linear against their formulas in 64 bits.
+
+Tolerances come from the arithmetic, element by element. A sum of K products in fp32 is off by at most
+(K + 8) 2^-23 sum |x||w| whatever its order (a whole step per addition); a mean or variance over a group of
+`count` values, summed by 64 threads or more, by (count / 64 + 64) 2^-23 relative to the mean of the summed
+magnitudes. Activations have slope at most 1.13 and are evaluated to 2^-20 |y| + 2^-22 |v|; the store rounds by
+half a step of the type.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from distributed_machine_learning_amd import ops  # noqa: E402
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+ACTS = ("none", "relu", "silu", "gelu", "gelu_tanh")
+U = 2.0 ** -23
+
+
+def act64(v, act):
+    if act == "relu":
+        return v.clamp(min=0)
+    if act == "silu":
+        return v * torch.sigmoid(v)
+    if act == "gelu":
+        return v * torch.special.ndtr(v)
+    if act == "gelu_tanh":
+        return v * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3))
+    return v
+
+
+def close(got, want, err, v=None):
+    """got within half a step of its type plus err (1.13 err behind an activation of v) of want."""
+    if v is not None:
+        err = 1.13 * err + 2.0 ** -20 * want.abs() + 2.0 ** -22 * v.abs()
+    half = torch.finfo(got.dtype).eps / 2
+    tol = half * (want.abs() + err) + err + torch.finfo(got.dtype).tiny
+    off = (got.double() - want).abs()
+    assert not got.isnan().any()
+    worst = (off / tol).max().item() if got.numel() else 0.0
+    assert worst <= 1.0, f"{worst:.3g} times the tolerance, off by {off.max().item():.3g}"
+
+
+def gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def normal(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+# ---------------------------------------------------------------- group norm
+
+
+def norm64(x, groups, weight, bias, eps, act):
+    """(y, v, err): the formula in 64 bits, its value before the activation, and how far fp32 may be off."""
+    n, c = x.shape[0], x.shape[-1]
+    xd = x.double().reshape(n, -1, groups, c // groups)
+    count = xd.shape[1] * xd.shape[3]
+    mu = xd.mean((1, 3), keepdim=True)
+    var = (xd - mu).square().mean((1, 3), keepdim=True)
+    rs = 1 / torch.sqrt(var + eps)
+    d = (count / 64 + 64) * U
+    # |mu' - mu| <= d mean|x|; the centred values carry that and a step of x; the variance carries their square
+    emu = d * xd.abs().mean((1, 3), keepdim=True)
+    ec = emu + U * (xd.abs() + mu.abs())
+    evar = d * (var + emu ** 2) + emu ** 2 + 2 * U * xd.abs().amax((1, 3), keepdim=True) * var.sqrt()
+    # the relative error of 1/sqrt(var + eps), which stays below 1/sqrt(eps) however far var is off
+    rel = (evar / (var + eps)).clamp(max=1) + 4 * U
+    xhat = (xd - mu) * rs
+    err = (ec * rs * (1 + rel) + xhat.abs() * (rel + 4 * U)).reshape(x.shape)
+    xhat = xhat.reshape(x.shape)
+    w = torch.ones(c, device=x.device, dtype=torch.double) if weight is None else weight.double()
+    b = torch.zeros(c, device=x.device, dtype=torch.double) if bias is None else bias.double()
+    v = xhat * w + b
+    return act64(v, act), v, err * w.abs() + 2 * U * ((xhat * w).abs() + b.abs())
+
+
+def check_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", out=None):
+    y, v, err = norm64(x, groups, weight, bias, eps, act)
+    got = ops.group_norm(x, groups, weight, bias, eps, act=act, out=out)
+    assert got.shape == x.shape and got.dtype is x.dtype
+    close(got, y, err, v)
+    return got
+
+
+NORM_SHAPES = [
+    # shape, groups
+    ((1, 1, 1), 1), ((2, 1, 8), 8), ((3, 5, 6), 3), ((1, 14, 14, 512), 32), ((2, 35, 35, 288), 32),
+    ((8, 197, 768), 32), ((2, 7, 7, 2048), 32), ((2, 9, 64), 1), ((5, 33, 66), 2), ((2, 3, 4, 5, 48), 16),
+    ((2, 56, 56, 256), 32), ((1, 4096, 64), 64), ((3, 8), 2), ((1, 70000, 12), 3), ((40, 2, 40), 4),
+    ((1, 73, 74, 2048), 32), ((2, 1000, 320), 32), ((1, 2, 8192), 1), ((2, 130, 130, 24), 2), ((700, 3, 32), 4),
+    ((2, 31, 33), 33), ((1, 28, 28, 1000), 8), ((64, 56, 56, 64), 32),
+]
+
+
+@pytest.mark.parametrize("dtype", (BF, HF, FP))
+@pytest.mark.parametrize("shape, groups", NORM_SHAPES)
+def test_group_norm(shape, groups, dtype):
+    g = gen(sum(shape) + groups)
+    c = shape[-1]
+    x = (normal(g, *shape) * (0.5 * normal(g, c)).exp() + normal(g, c)).to(dtype)
+    act = ACTS[(shape[0] + c + groups) % 5]
+    check_norm(x, groups, 1 + 0.2 * normal(g, c), 0.2 * normal(g, c), act=act)
+
+
+@pytest.mark.parametrize("dtype", (BF, FP))
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape, groups", [((2, 10, 10, 64), 8), ((2, 13, 35), 5), ((1, 9000, 96), 12)])
+def test_group_norm_acts_and_parameters(shape, groups, act, dtype):
+    g = gen(7)
+    c = shape[-1]
+    x = (3 * normal(g, *shape)).to(dtype)
+    check_norm(x, groups, act=act)
+    check_norm(x, groups, normal(g, c).to(dtype), None, act=act)
+    check_norm(x, groups, None, normal(g, 2 * c)[::2], eps=0.5, act=act)
+
+
+@pytest.mark.parametrize("dtype", (BF, HF, FP))
+@pytest.mark.parametrize("c, pitch, off", [(64, 96, 32), (64, 64, 0), (64, 67, 3), (24, 33, 1), (288, 384, 96),
+                                           (40, 44, 4), (32, 34, 2)])
+def test_group_norm_slices(c, pitch, off, dtype):
+    """A channel slice of a wider buffer, into one of another: nothing else is read into it or written."""
+    g = gen(3)
+    buf = torch.full((3, 11, 13, pitch), float("nan"), device="cuda", dtype=dtype)
+    buf[..., off:off + c] = normal(g, 3, 11, 13, c).to(dtype)
+    wide = torch.full((3, 11, 13, pitch + 5), 7.0, device="cuda", dtype=dtype)
+    check_norm(buf[..., off:off + c], 8, normal(g, c), normal(g, c), act="silu", out=wide[..., 2:2 + c])
+    assert (wide[..., :2] == 7).all() and (wide[..., 2 + c:] == 7).all()
+    check_norm(buf[::2, :, :, off:off + c], 4)        # a pitch between samples of its own
+    check_norm(buf[1:2, 2:3, :, off:off + c], 4)
+    x = buf[..., off:off + c]
+    want = ops.group_norm(x, 8, act="gelu")
+    assert ops.group_norm(x, 8, act="gelu", out=x) is x and torch.equal(x, want)  # in place
+
+
+@pytest.mark.parametrize("shape, groups", [((2, 50, 64), 8), ((1, 9000, 96), 3), ((2, 20, 35), 5)])
+def test_group_norm_level_far_above_spread(shape, groups):
+    """Spread 1 at a level of 1000: a variance from E[x^2] - mu^2 would have lost it."""
+    g = gen(11)
+    check_norm(1000 + normal(g, *shape), groups)
+    check_norm((200 + 8 * normal(g, *shape)).to(BF), groups)
+    y = ops.group_norm(torch.full(shape, 1000.0, device="cuda"), groups, bias=torch.full((shape[-1],), 0.5, device="cuda"))
+    assert (y == 0.5).all()  # equal values: exactly the bias
+
+
+@pytest.mark.parametrize("bad", (float("nan"), float("inf"), -float("inf")))
+@pytest.mark.parametrize("shape, groups", [((2, 50, 64), 8), ((2, 9000, 96), 4), ((3, 20, 35), 5)])
+def test_group_norm_keeps_bad_values_to_their_group(shape, groups, bad):
+    g = gen(13)
+    x = normal(g, *shape).to(BF)
+    per = shape[-1] // groups
+    want = ops.group_norm(x, groups, act="silu")
+    x[1, 7, per + 1] = bad
+    y = ops.group_norm(x, groups, act="silu")
+    hit = torch.zeros(shape, dtype=torch.bool, device="cuda")
+    hit[1, :, per:2 * per] = True
+    assert y[hit].isnan().all() and torch.equal(y[~hit], want[~hit])
+    assert ops.group_norm(x, groups, act="relu")[hit].isnan().all()
+
+
+def test_group_norm_empty():
+    for shape in ((0, 4, 8), (2, 0, 8)):
+        assert ops.group_norm(torch.empty(shape, device="cuda", dtype=BF), 2).shape == shape
+
+
+def test_group_norm_offsets_beyond_32_bits():
+    """Samples further apart than 2^31 elements."""
+    g = gen(17)
+    buf = torch.empty(2 ** 31 + 64 * 50, device="cuda", dtype=BF)
+    x = buf.as_strided((2, 50, 64), (2 ** 31, 64, 1))
+    x.copy_(normal(g, 2, 50, 64))
+    check_norm(x, 8)
+    y = torch.empty(2 ** 31 + 64 * 50, device="cuda", dtype=BF).as_strided((2, 50, 64), (2 ** 31, 64, 1))
+    check_norm(x, 8, out=y)
+
+
+# ---------------------------------------------------------------- products
+
+
+def rows64(x, w, b, r, act, last):
+    """(y, v, err) of rows that share one weight, in 64 bits."""
+    xd, wd = x.double(), w.double()
+    v = xd @ wd.t()
+    err = (x.shape[-1] + 8) * U * (xd.abs() @ wd.abs().t())
+    if b is not None:
+        v = v + b.double()
+        err = err + 2 * U * v.abs()
+    if r is not None and last:
+        v = v + r.double()
+        err = err + 2 * U * v.abs()
+    y = act64(v, act)
+    if r is not None and not last:
+        err = err + 2 * U * r.double().abs()
+        y = y + r.double()
+        v = v.abs() + r.double().abs()
+    return y, v, err
+
+
+def check_linear(x, w, b=None, act="none", r=None, last=False, **kw):
+    x2 = x.reshape(-1, x.shape[-1])
+    y, v, err = rows64(x2, w, b, None if r is None else r.reshape(-1, w.shape[0]), act, last)
+    got = ops.linear(x, w, b, act=act, residual=r, act_last=last, **kw)
+    assert got.shape == (*x.shape[:-1], w.shape[0])
+    close(got.reshape(y.shape), y, err, v)
+    return got
+
+
+def operands(g, m, k, n, dtype):
+    return normal(g, m, k).to(dtype), (normal(g, n, k) * max(1, k) ** -0.5).to(dtype), 0.5 * normal(g, n)
+
+
+SIZES = [(1, 1, 1), (1, 16, 1000), (1, 2048, 1000), (1, 4099, 33), (2, 64, 64), (3, 100, 17), (16, 512, 256),
+         (17, 520, 264), (31, 1024, 48), (64, 64, 64), (65, 33, 129), (100, 2048, 100), (128, 4096, 512),
+         (200, 72, 4096), (256, 256, 256), (257, 1000, 257), (333, 1001, 517), (512, 128, 1024), (1000, 768, 776),
+         (1, 8192, 8192), (5, 8191, 1023), (2000, 8, 40), (700, 2056, 520), (2049, 192, 264), (4100, 64, 8)]
+
+
+@pytest.mark.parametrize("dtype", (BF, HF))
+@pytest.mark.parametrize("m, k, n", SIZES)
+def test_linear(m, k, n, dtype):
+    g = gen(m + k + n)
+    x, w, b = operands(g, m, k, n, dtype)
+    act = ACTS[(m + n) % 5]
+    check_linear(x, w, b, act)
+    check_linear(x, w, b, act, out_dtype=FP)
+    r = normal(g, m, n)
+    check_linear(x, w, None, act, r.to(dtype), last=bool(n % 2))
+    check_linear(x, w, b, act, r, last=not n % 2, out_dtype=FP)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("last", (False, True))
+@pytest.mark.parametrize("m, k, n", [(2, 256, 64), (300, 128, 320)])
+def test_linear_epilogues(m, k, n, act, last):
+    g = gen(5)
+    x, w, b = operands(g, m, k, n, BF)
+    r = normal(g, m, n)
+    check_linear(4 * x, w, b, act, r.to(BF), last)
+    check_linear(4 * x, w, b.to(BF), act, normal(g, n).expand(m, n), last, out_dtype=FP)  # a broadcast residual
+    want = ops.linear(x, w, b, act=act, residual=r, act_last=last, out_dtype=FP)
+    assert ops.linear(x, w, b, act=act, residual=r, act_last=last, out=r) is r and torch.equal(r, want)
+
+
+@pytest.mark.parametrize("dtype", (BF, HF))
+@pytest.mark.parametrize("pad, off", [(0, 0), (8, 8), (1, 0), (1, 1), (2, 2), (3, 1), (64, 4)])
+@pytest.mark.parametrize("m, k, n", [(1, 512, 100), (7, 130, 40), (50, 64, 72), (300, 256, 264), (290, 257, 130),
+                                     (300, 320, 256)])
+def test_linear_strides(m, k, n, pad, off, dtype):
+    """Columns of wider buffers on every side, of any alignment, NaN in the rest of them."""
+    g = gen(19)
+
+    def inside(t):
+        wide = torch.full((t.shape[0] + 2, t.shape[1] + pad + off), float("nan"), device="cuda", dtype=t.dtype)
+        view = wide[1:-1, off:off + t.shape[1]]
+        view.copy_(t)
+        return view
+
+    x, w, b = operands(g, m, k, n, dtype)
+    out = torch.full((m + 2, n + pad + off), 7.0, device="cuda", dtype=dtype)
+    check_linear(inside(x), inside(w), b, "relu", inside(normal(g, m, n).to(dtype)), out=out[1:-1, off:off + n])
+    out[1:-1, off:off + n] = 7
+    assert (out == 7).all()
+
+
+def test_linear_shapes():
+    g = gen(23)
+    x, w, b = operands(g, 24, 32, 48, BF)
+    for shape in ((32,), (1, 32), (2, 3, 4, 32), (24, 1, 32)):
+        check_linear(x.reshape(-1)[:math.prod(shape)].view(shape), w, b)
+    assert ops.linear(x[:0], w, b).shape == (0, 48)
+    assert ops.linear(x, w[:0]).shape == (24, 0)
+    got = ops.linear(x[:, :0], w[:, :0], b, act="relu", out_dtype=FP)  # an empty sum: the bias
+    assert torch.equal(got, b.clamp(min=0).expand(24, 48))
+    assert (ops.linear(x[:, :0], w[:, :0]) == 0).all()
+
+
+def test_linear_keeps_bad_values_to_their_row():
+    g = gen(29)
+    for m, k, n in ((3, 100, 70), (300, 136, 264), (40, 512, 64)):
+        x, w, b = operands(g, m, k, n, BF)
+        want = ops.linear(x, w, b, act="silu")
+        x[1, k - 1] = float("nan")
+        x[2, 0] = float("inf")
+        got = ops.linear(x, w, b, act="silu")
+        assert got[1].isnan().all() and ((~got[2].isfinite()) | (got[2] == 0)).all()
+        keep = torch.arange(m, device="cuda") != 1
+        keep[2] = False
+        assert torch.equal(got[keep], want[keep])
+        assert ops.linear(x, w, b, act="relu")[1].isnan().all()
+
+
+def test_linear_offsets_beyond_32_bits():
+    """Rows further apart than 2^31 bytes on every side, and more than 2^31 elements between the first and last."""
+    g = gen(31)
+    step = 2 ** 30 + 8
+    x, w, b = operands(g, 4, 64, 80, BF)
+    buf = torch.empty(3 * step + 80, device="cuda", dtype=BF)
+    far = buf.as_strided((4, 64), (step, 1))
+    far.copy_(x)
+    want = ops.linear(x, w, b)
+    assert torch.equal(ops.linear(far, w, b), want)
+    out = buf.as_strided((4, 80), (step, 1))
+    assert torch.equal(ops.linear(x, w, b, out=out), want)
+    buf.as_strided((4, 64), (step, 1)).copy_(w[:4])
+    assert torch.equal(ops.linear(x, buf.as_strided((4, 64), (step, 1)), b[:4]), want[:, :4])
+
+
+# ---------------------------------------------------------------- grouped products
+
+
+def spans(ends, t):
+    """The rows of each group: the ends clamped to an ascending sequence in [0, t]."""
+    at, got = 0, []
+    for e in ends:
+        e = max(at, min(max(e, 0), t))
+        got.append((at, e))
+        at = e
+    return got, at
+
+
+def check_grouped(g, sizes, k, n, dtype, act="none", spare=0, residual=False, last=False, out_dtype=None, ends=None,
+                  wide=torch.int32, x=None):
+    t = sum(sizes) + spare
+    e = len(sizes)
+    x = normal(g, t, k).to(dtype) if x is None else x
+    w = (normal(g, e, n, k) * max(1, k) ** -0.5).to(dtype)
+    b = 0.5 * normal(g, e, n)
+    to = out_dtype or dtype
+    r = normal(g, t, n).to(to) if residual else None
+    if ends is None:
+        ends = torch.tensor(sizes).cumsum(0).tolist()
+    dev = torch.tensor(ends, device="cuda", dtype=wide)
+    out = torch.full((t, n), 7.0, device="cuda", dtype=to)
+    got = ops.grouped_linear(x, w, dev, b, act=act, residual=r, act_last=last, out=out)
+    assert got is out
+    pieces, rows = spans(ends, t)
+    for i, (p, q) in enumerate(pieces):
+        if q > p:
+            y, v, err = rows64(x[p:q], w[i], b[i], None if r is None else r[p:q], act, last)
+            close(got[p:q], y, err, v)
+    assert (got[rows:] == 7).all()
+    fresh = ops.grouped_linear(x, w, dev, b, act=act, residual=r, act_last=last, out_dtype=out_dtype)
+    assert torch.equal(fresh[:rows], got[:rows]) and (fresh[rows:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", (BF, HF))
+@pytest.mark.parametrize("sizes, k, n", [
+    ([5], 64, 64), ([0, 0, 0], 32, 16), ([0, 3, 0, 1, 0], 256, 100), ([1] * 70, 64, 40), ([0] * 130 + [9], 40, 33),
+    ([64, 64], 128, 128), ([63, 65, 1], 128, 136), ([300, 0, 17, 511, 2], 192, 264), ([2, 1, 0, 4] * 50, 72, 24),
+    ([33, 54, 51, 13, 0, 49], 513, 250), ([700, 1, 1300], 64, 520), ([16] * 8, 1024, 512), ([257], 1000, 300),
+    ([1, 0, 1, 1, 0, 0, 2, 1], 2048, 512), ([129, 40], 4096, 72)])
+def test_grouped_linear(sizes, k, n, dtype):
+    g = gen(sum(sizes) + k)
+    i = (len(sizes) + n) % 5
+    check_grouped(g, sizes, k, n, dtype, ACTS[i])
+    check_grouped(g, sizes, k, n, dtype, ACTS[(i + 1) % 5], spare=70, residual=True, last=bool(k % 3), wide=torch.int64)
+    check_grouped(g, sizes, k, n, dtype, ACTS[(i + 2) % 5], spare=1, residual=True, out_dtype=FP)
+
+
+@pytest.mark.parametrize("k, n", [(64, 96), (1024, 24), (33, 17)])
+@pytest.mark.parametrize("ends", [[9, 3, 20, 12], [-5, 4, 1000, 8], [2 ** 31 - 1, 0, 0, 0], [-2 ** 31, -1, 7, 7],
+                                  [40, 40, 40, 40], [0, 0, 0, 0]])
+def test_grouped_linear_clamps_ends(ends, k, n):
+    g = gen(37)
+    check_grouped(g, [10] * 4, k, n, BF, "gelu", ends=ends)
+    check_grouped(g, [300] * 4, k, n, BF, "gelu", ends=[30 * e for e in ends], wide=torch.int64)
+
+
+def test_grouped_linear_ignores_rows_behind_the_last():
+    g = gen(41)
+    x = normal(g, 400, 72).to(BF)
+    x[150:] = float("nan")
+    check_grouped(g, [100, 0, 50], 72, 80, BF, "silu", spare=250, x=x)
+
+
+def test_grouped_linear_empty():
+    z = torch.zeros
+    kw = {"device": "cuda", "dtype": BF}
+    none = z(0, device="cuda", dtype=torch.int32)
+    assert ops.grouped_linear(z(0, 8, **kw), z(2, 6, 8, **kw), z(2, device="cuda", dtype=torch.int32)).shape == (0, 6)
+    assert (ops.grouped_linear(z(3, 8, **kw), z(0, 6, 8, **kw), none) == 0).all()
+    out = torch.full((3, 6), 7.0, **kw)
+    assert (ops.grouped_linear(z(3, 8, **kw), z(0, 6, 8, **kw), none, out=out) == 7).all()
+    ends = torch.tensor([1, 3], device="cuda")
+    b = torch.ones(2, 6, device="cuda") * torch.tensor([[2.0], [3.0]], device="cuda")
+    got = ops.grouped_linear(z(4, 0, **kw), z(2, 6, 0, **kw), ends, b)  # empty sums: each group's bias
+    assert got[:, 0].tolist() == [2, 3, 3, 0]
+
+
+def test_grouped_linear_rows_match_linear_of_their_group():
+    """Strided weights (a slice of a wider stack), and the same rows through linear one group at a time."""
+    g = gen(43)
+    stack = (normal(g, 3, 2, 136, 200) * 0.1).to(BF)
+    w = stack[:, 1, :128, 8:136]
+    x = normal(g, 90, 128).to(BF)
+    ends = torch.tensor([30, 31, 90], device="cuda")
+    got = ops.grouped_linear(x, w, ends, act="silu", out_dtype=FP)
+    at = 0
+    for e, end in enumerate((30, 31, 90)):
+        y, v, err = rows64(x[at:end], w[e], None, None, "silu", False)
+        close(got[at:end], y, err, v)
+        at = end
+
+
+# ---------------------------------------------------------------- streams, graphs, together
+
+
+def block(x, p):
+    """Norm and product of a residual block, a head per group of rows, and the framework's top-5 behind it."""
+    h = ops.group_norm(x, 8, p["gw"], p["gb"], act="silu")
+    h = ops.linear(h, p["w1"], p["b1"], act="gelu")
+    y = ops.linear(h, p["w2"], p["b2"], residual=x)
+    h = ops.conv2d_nhwc(ops.group_norm(y, 8, act="relu"), p["wc"], p["bc"], 64, 3, 3, pad=(1, 1), relu=True)
+    f = ops.global_avgpool(h)
+    logits = ops.grouped_linear(f, p["heads"], p["ends"], p["hb"], out_dtype=FP)
+    return y, logits, ops.softmax_top5(logits)
+
+
+def block_parameters(g):
+    wc = normal(g, 64, 64, 3, 3) * 24 ** -1.0
+    return {"gw": 1 + 0.1 * normal(g, 64), "gb": 0.1 * normal(g, 64),
+            "w1": (normal(g, 256, 64) / 8).to(BF), "b1": 0.1 * normal(g, 256),
+            "w2": (normal(g, 64, 256) / 16).to(BF), "b2": 0.1 * normal(g, 64),
+            "wc": ops.pack_weight(wc)[0].cuda(), "bc": 0.1 * normal(g, 64), "wc4": wc.to(BF),
+            "heads": (normal(g, 3, 120, 64) / 8).to(BF), "hb": normal(g, 3, 120),
+            "ends": torch.tensor([2, 2, 5], device="cuda", dtype=torch.int32)}
+
+
+def test_block_with_the_framework_s_operators():
+    g = gen(47)
+    p, x = block_parameters(g), normal(g, 5, 12, 12, 64).to(BF)
+    y, logits, (probs, idx, top) = block(x, p)
+    # the same in 64 bits, rounded to bf16 where the operators hand on bf16
+    def bf(t):
+        return t.to(BF).double()
+    h = bf(norm64(x, 8, p["gw"], p["gb"], 1e-5, "silu")[0])
+    h = bf(act64(h @ p["w1"].double().t() + p["b1"].double(), "gelu"))
+    y64 = h @ p["w2"].double().t() + p["b2"].double() + x.double()
+    # three roundings to bf16 ahead of y: each moves a product's sum by at most 2^-8 of its terms' magnitudes
+    assert ((y.double() - y64).norm() / y64.norm()).item() < 3 * 2.0 ** -8
+    h = bf(norm64(y, 8, None, None, 1e-5, "relu")[0])
+    c = torch.nn.functional.conv2d(h.permute(0, 3, 1, 2), p["wc4"].double(), p["bc"].double(), padding=1).clamp(min=0)
+    f = bf(bf(c).mean((2, 3)))
+    want = torch.stack([f[i] @ p["heads"][e].double().t() + p["hb"][e].double() for i, e in enumerate((0, 0, 2, 2, 2))])
+    assert ((logits.double() - want).norm() / want.norm()).item() < 4 * 2.0 ** -8
+    assert torch.equal(idx[:, 0].long(), logits.argmax(1))
+    assert torch.allclose(probs, logits.softmax(1), atol=1e-5)
+
+
+@pytest.mark.parametrize("m", (1, 40, 700))
+def test_replayed_graph_follows_its_inputs(m):
+    """Captured calls on new inputs, group ends among them, over several replays with eager work in between."""
+    g = gen(53)
+    x, w, b = operands(g, m, 1032, 264, BF)
+    stack = torch.stack([w, 2 * w, -w])
+    ends = torch.tensor([m // 3, m // 2, m], device="cuda", dtype=torch.int32)
+    img = normal(g, 2, 40 * m, 96).to(BF)
+
+    def calls():
+        return (ops.linear(x, w, b, act="gelu"), ops.grouped_linear(x, stack, ends, act="silu", out_dtype=FP),
+                ops.group_norm(img, 6, act="relu"), ops.linear(x[:1], w, b))
+
+    calls()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs of the same calls, replayed one behind the other
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = calls()
+        graphs.append((graph, out))
+    for i in range(4):
+        x.copy_(normal(g, *x.shape))
+        img.copy_(normal(g, *img.shape))
+        ends.copy_(torch.tensor([[m, m, m], [0, m // 2, m], [0, 0, m // 2 + 1], [1, 1, m]][i]))
+        want = [t.clone() for t in calls()]
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            for a, c in zip(out, want):
+                assert torch.equal(a, c)
+
+
+def test_calls_on_two_streams():
+    g = gen(59)
+    x, w, b = operands(g, 40, 4096, 264, BF)
+    img = normal(g, 1, 20000, 96).to(BF)
+    want = (ops.linear(x, w, b), ops.group_norm(img, 6))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((ops.linear(x, w, b), ops.group_norm(img, 6)))
+    torch.cuda.synchronize()
+    for a, c in got:
+        assert torch.equal(a, want[0]) and torch.equal(c, want[1])
+
+
+def test_repeats_are_bit_identical():
+    g = gen(61)
+    x, w, b = operands(g, 150, 4096, 200, HF)
+    img = normal(g, 3, 5000, 96)
+    want = (ops.linear(x, w, b), ops.group_norm(img, 6))
+    for _ in range(5):
+        assert torch.equal(ops.linear(x, w, b), want[0]) and torch.equal(ops.group_norm(img, 6), want[1])
