@@ -184,6 +184,8 @@ typedef struct {
   const float* weight;  // fp32 [C] or null (1)
   const float* bias;    // fp32 [C] or null (0)
   int64_t xn, yn, ldx, ldy;
+  void* ws;             // dml_group_norm_workspace() bytes, used until the call's last kernel is done
+  int64_t ws_bytes;
   int N, HW, C, G;
   int dtype, act;
   float eps;
@@ -266,6 +268,7 @@ int dml_softmax_top5(const float* logits, int B, int classes, int ld, float* pro
 int dml_softmax_top5_split(float* logits, int B, int classes, int ld, int nsplit, int split_ld,
                            float* probs_out, int* top_idx, float* top_p, hipStream_t s);
 int dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s);
+int64_t dml_group_norm_workspace(const DmlGroupNormArgs* a);  // 0: none needed, -1: arguments refused
 int dml_product(const DmlProductArgs* a, hipStream_t s);
 int dml_preprocess(const DmlPreprocArgs* a, hipStream_t s);
 int dml_index_fetch(const int* host, int* dev, int n, hipStream_t s);  // pinned host table -> device

@@ -54,6 +54,8 @@ def _flags() -> list[str]:
         "-fPIC",
         "-mcode-object-version=5",
         "-munsafe-fp-atomics",
+        # no packed fp32 arithmetic: some of its forms have given wrong results on this card
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         f"-I{CSRC / 'include'}",
         f"-I{CSRC / 'kernels'}",
     ]

@@ -102,6 +102,7 @@ class GroupNormArgs(C.Structure):
     _fields_ = [
         ("x", C.c_void_p), ("y", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
         ("xn", C.c_int64), ("yn", C.c_int64), ("ldx", C.c_int64), ("ldy", C.c_int64),
+        ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
         ("N", C.c_int), ("HW", C.c_int), ("C", C.c_int), ("G", C.c_int),
         ("dtype", C.c_int), ("act", C.c_int), ("eps", C.c_float),
     ]
@@ -121,6 +122,7 @@ class ProductArgs(C.Structure):
 
 _SIGS = {
     "dml_group_norm": (C.c_int, [C.POINTER(GroupNormArgs), C.c_void_p]),
+    "dml_group_norm_workspace": (C.c_int64, [C.POINTER(GroupNormArgs)]),
     "dml_product": (C.c_int, [C.POINTER(ProductArgs), C.c_void_p]),
     "dml_expand_reduce": (C.c_int, [C.POINTER(ExpandReduceArgs), C.c_void_p]),
     "dml_chain_supported": (C.c_int, [C.POINTER(ExpandReduceArgs)]),

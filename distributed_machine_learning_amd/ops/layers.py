@@ -148,7 +148,11 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         bias = bias.float().contiguous()
     a = N.GroupNormArgs(x.data_ptr(), out.data_ptr(), weight.data_ptr() if weight is not None else None,
                         bias.data_ptr() if bias is not None else None, x.stride(0), out.stride(0),
-                        ldx, ldy, n, rows, c, groups, _DTYPES[x.dtype], code, eps)
+                        ldx, ldy, None, 0, n, rows, c, groups, _DTYPES[x.dtype], code, eps)
+    a.ws_bytes = N.check(N.lib().dml_group_norm_workspace(C.byref(a)), "dml_group_norm_workspace")
+    if a.ws_bytes:
+        ws = torch.empty(a.ws_bytes, device=x.device, dtype=torch.uint8)
+        a.ws = ws.data_ptr()
     _launch(N.lib().dml_group_norm, a, x.device, "dml_group_norm")
     return out
 
