@@ -184,7 +184,7 @@ typedef struct {
   const float* weight;  // fp32 [C] or null (1)
   const float* bias;    // fp32 [C] or null (0)
   int64_t xn, yn, ldx, ldy;
-  void* ws;             // dml_group_norm_workspace() bytes, used until the call's last kernel is done
+  void* ws;             // scratch of the call's kernels, ws_bytes long (the size: dml_group_norm's answer without)
   int64_t ws_bytes;
   int N, HW, C, G;
   int dtype, act;
@@ -267,8 +267,8 @@ int dml_softmax_top5(const float* logits, int B, int classes, int ld, float* pro
 // slice 0 before the softmax.
 int dml_softmax_top5_split(float* logits, int B, int classes, int ld, int nsplit, int split_ld,
                            float* probs_out, int* top_idx, float* top_p, hipStream_t s);
-int dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s);
-int64_t dml_group_norm_workspace(const DmlGroupNormArgs* a);  // 0: none needed, -1: arguments refused
+// -1: refused; > 0: nothing was launched, call again with a workspace of this many bytes
+int64_t dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s);
 int dml_product(const DmlProductArgs* a, hipStream_t s);
 int dml_preprocess(const DmlPreprocArgs* a, hipStream_t s);
 int dml_index_fetch(const int* host, int* dev, int n, hipStream_t s);  // pinned host table -> device

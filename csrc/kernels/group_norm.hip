@@ -9,8 +9,8 @@
 // is a run of S channels. A thread keeps one column of vectors, hence one set of channels,
 // weights and groups, and walks the rows.
 //
-//  * one_pass: the slab stays in registers between its one read and its one write, up to 16
-//    vectors in each of 1024 threads (256 KiB).
+//  * one_pass: the slab stays in registers (and, for the longest, LDS) between its one read and
+//    its one write: up to 400 KiB in a workgroup.
 //  * stats + apply: slabs beyond that, or too few slabs to fill the card. Every chunk of rows
 //    yields (mean, sum of squared distances from it) per group in the workspace; the second
 //    kernel merges the chunks and reads x again.
@@ -23,175 +23,229 @@
 namespace dml {
 namespace gn {
 
+typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kMaxGroups = 256;  // groups of a slab
 
-// How a slab lies over NT threads.
+// t / d for 0 <= t < 2^21: t + 1/2 is at least 1/(2d) away from a multiple of d, the reciprocal's error below that
+__device__ __forceinline__ int div_small(int t, float inv) { return (int)(((float)t + 0.5f) * inv); }
+
+// How a slab of S >= V channels lies over NT threads.
 template <class T, int NT, bool CH>
 struct Slab {
   static constexpr int V = Vec16<T>::N;
-  static constexpr int PC = CH ? V : 1;  // partial sums of a thread: per channel, or one where a vector is in one group
-  int S, cg, cols, gs, RT, rt, col, n;   // channels, group width, vector columns, groups, row threads; mine; valid channels
+  static constexpr int PC = CH ? V : 1;  // statistics of a thread: per channel, or one where a vector is in one group
+  int S, cg, cols, gs, RT;  // channels, group width, vector columns, groups, row threads
+  int rt, c, lo;            // this thread's first row, first channel, own channels [lo, V) of the vector there
   bool on;
   __device__ __forceinline__ Slab(int S_, int cg_) : S(S_), cg(cg_) {
     cols = (S + V - 1) / V;
     gs = S / cg;
-    RT = NT / cols;
-    rt = threadIdx.x / cols;
-    col = threadIdx.x - rt * cols;
+    RT = div_small(NT, __builtin_amdgcn_rcpf((float)cols));
+    rt = div_small(threadIdx.x, __builtin_amdgcn_rcpf((float)cols));
+    const int col = threadIdx.x - rt * cols;
     on = rt < RT;
-    n = min(V, S - col * V);
+    // the last vector ends with the slab: where V does not divide S it shares channels with the one before it (both
+    // load and store them, with the same values; the statistics take them from that one)
+    c = min(col * V, S - V);
+    lo = col * V - c;
   }
-  // Sums of v over the slab's groups -> stat[0 .. gs): every thread leaves its partial sums in
-  // LDS, then one wave per group adds the group's in a fixed order.
-  __device__ __forceinline__ void sum(const float (&v)[PC], float* part, float* stat) const {
-    if (on) {
-#pragma unroll
-      for (int p = 0; p < PC; ++p) part[threadIdx.x * PC + p] = v[p];
-    }
-    __syncthreads();
-    const int lane = threadIdx.x & 63, SW = cols * PC, gw = CH ? cg : cg / V;
-    for (int g = threadIdx.x >> 6; g < gs; g += NT / 64) {
-      float s = 0.f;
-      for (int t = lane; t < RT * gw; t += 64) {
-        const int r = t / gw;
-        s += part[r * SW + g * gw + t - r * gw];
-      }
-#pragma unroll
-      for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-      if (lane == 0) stat[g] = s;
-    }
-    __syncthreads();
+  // rows r, r + RT, ... below `rows` (at most 64 a thread)
+  __device__ __forceinline__ int rows_of(int r, int rows) const {
+    return r < rows ? 1 + div_small(rows - 1 - r, __builtin_amdgcn_rcpf((float)RT)) : 0;
   }
-  // stat of this thread's channels (PC of them)
+  // The group's statistic at this thread's channels.
   __device__ __forceinline__ void mine(const float* stat, float (&f)[PC]) const {
+    const float inv = __builtin_amdgcn_rcpf((float)cg);
 #pragma unroll
-    for (int p = 0; p < PC; ++p) f[p] = stat[min((col * V + p) / cg, gs - 1)];
-  }
-  __device__ __forceinline__ void load(Vec16<T>& v, const T* p) const {
-    if (n == V) v.load(p);
-    else v.load(p, n);
-  }
-  __device__ __forceinline__ void store(const Vec16<T>& v, T* p) const {
-    if (n == V) v.store(p);
-    else v.store(p, n);
+    for (int p = 0; p < PC; ++p) f[p] = stat[min(div_small(c + p, inv), gs - 1)];
   }
 };
+
+// A thread's vectors: R in registers, RL in LDS (its own 16 bytes of each row of lds).
+template <class T, int NT, int R, int RL>
+struct Held {
+  Vec16<T> v[R];
+  template <class F>
+  __device__ __forceinline__ void each(int count, char* lds, F f) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (i < count) f(v[i], i);
+    if constexpr (RL > 0) {
+      for (int i = R; i < count; ++i) {
+        Vec16<T> t;
+        __builtin_memcpy(&t.v, lds + ((i - R) * NT + threadIdx.x) * 16, 16);
+        f(t, i);
+      }
+    }
+  }
+};
+
+// Rows [0, rows) of the slab into registers and LDS; the groups' means -> stat[0 .. gs), their sums of squared
+// distances from it -> stat[kMaxGroups ...). Each thread centres its own values (its mean, then its M2: no
+// barrier), leaves the pair in LDS, and one wave per group merges the group's pairs in a fixed order.
+template <class T, int NT, int R, int RL, bool ONCE, bool CH, class F>
+__device__ __forceinline__ void read_and_sum(const Slab<T, NT, CH>& s, const T* x, int64_t ldx, int rows,
+                                             Held<T, NT, R, RL>& h, int count, char* lds, float2* part, float* stat,
+                                             F meanwhile) {
+  constexpr int V = Vec16<T>::N, PC = Slab<T, NT, CH>::PC;
+  x += s.rt * ldx;
+  const int64_t step = s.RT * ldx;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < count) {
+      if constexpr (ONCE) h.v[i].load_once(x + i * step);
+      else h.v[i].load(x + i * step);
+    }
+  if constexpr (RL > 0) {
+#pragma unroll
+    for (int i = R; i < R + RL; ++i) {
+      if (i >= count) continue;
+      __builtin_amdgcn_global_load_lds((const void*)(x + i * step),
+                                       (lds_void*)(lds + ((i - R) * NT + (threadIdx.x & ~63)) * 16), 16, 0, 0);
+    }
+  }
+  if constexpr (RL > 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  float mean[PC] = {}, m2[PC] = {};
+  h.each(count, lds, [&](const Vec16<T>& v, int) {
+    float f[V];
+    v.get(f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) mean[PC == 1 ? 0 : j] += f[j];
+  });
+  const float inv = count > 0 ? 1.f / (float)(count * (V / PC)) : 0.f;
+#pragma unroll
+  for (int p = 0; p < PC; ++p) mean[p] *= inv;
+  h.each(count, lds, [&](const Vec16<T>& v, int) {
+    float f[V];
+    v.get(f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = f[j] - mean[PC == 1 ? 0 : j];
+      m2[PC == 1 ? 0 : j] += d * d;
+    }
+  });
+  meanwhile();  // loads for later, in flight over the barriers
+  if (s.on) {
+    if constexpr (CH) {
+#pragma unroll
+      for (int p = 0; p < PC; ++p)
+        if (p >= s.lo) part[s.rt * s.cols * PC + s.c + p] = make_float2(mean[p], m2[p]);
+    } else {
+      part[threadIdx.x] = make_float2(mean[0], m2[0]);
+    }
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63, SW = s.cols * PC, gw = CH ? s.cg : s.cg / V;
+  const float inv_gw = __builtin_amdgcn_rcpf((float)gw), total = (float)rows * (float)s.cg;
+  const int entries = s.RT * gw;
+  for (int g = threadIdx.x >> 6; g < s.gs; g += NT / 64) {
+    float sum = 0.f, q = 0.f;
+#pragma unroll 2
+    for (int t = lane; t < entries; t += 64) {
+      const int r = div_small(t, inv_gw);
+      sum += part[r * SW + g * gw + t - r * gw].x * (float)(s.rows_of(r, rows) * (V / PC));
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const float mu = sum / total;
+#pragma unroll 2
+    for (int t = lane; t < entries; t += 64) {
+      const int r = div_small(t, inv_gw);
+      const float2 e = part[r * SW + g * gw + t - r * gw];
+      q += e.y + (e.x - mu) * (e.x - mu) * (float)(s.rows_of(r, rows) * (V / PC));
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) q += __shfl_xor(q, o, 64);
+    if (lane == 0) {
+      stat[g] = mu;
+      stat[kMaxGroups + g] = q;
+    }
+  }
+  __syncthreads();
+}
 
 // weight and bias of a thread's channels; `scale` = weight / sqrt(var + eps)
 template <class T, int PC>
 struct Affine {
   static constexpr int V = Vec16<T>::N;
   float scale[V], shift[V], mu[PC];
-  __device__ __forceinline__ void load(const DmlGroupNormArgs& a, int c, int n) {
+  __device__ __forceinline__ void load(const DmlGroupNormArgs& a, int c) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      scale[j] = a.weight && j < n ? a.weight[c + j] : 1.f;
-      shift[j] = a.bias && j < n ? a.bias[c + j] : 0.f;
+      scale[j] = a.weight ? a.weight[c + j] : 1.f;
+      shift[j] = a.bias ? a.bias[c + j] : 0.f;
     }
-  }
-  __device__ __forceinline__ void apply(Vec16<T>& v, int act) const {
-    float f[V];
-    v.get(f);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = (f[j] - mu[PC == 1 ? 0 : j]) * scale[j] + shift[j];
-    activate(f, act);
-    v.set(f);
   }
 };
 
-// Rows [row0, row0 + rows) of the slab in registers; mean and M2 of its groups -> stat[0..gs), stat[kMaxGroups + ...)
-template <class T, int NT, int R, bool CH>
-__device__ __forceinline__ void read_and_sum(const Slab<T, NT, CH>& s, const T* x, int64_t ldx, int rows, float count,
-                                             Vec16<T> (&v)[R], float (&mu)[Slab<T, NT, CH>::PC], float* part,
-                                             float* stat) {
-  constexpr int V = Vec16<T>::N, PC = Slab<T, NT, CH>::PC;
-  float acc[PC] = {};
+// The held vectors through the affine map and the activation -> y
+template <int KIND, class T, int NT, int R, int RL, int PC>
+__device__ __forceinline__ void write_as(Held<T, NT, R, RL>& h, const Affine<T, PC>& f, Act act, int count, char* lds,
+                                         T* y, int64_t step) {
+  constexpr int V = Vec16<T>::N;
+  h.each(count, lds, [&](const Vec16<T>& v, int i) {
+    float u[V];
+    v.get(u);
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int r = s.rt + i * s.RT;
-    if (s.on && r < rows) s.load(v[i], x + (int64_t)r * ldx);
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (s.on && s.rt + i * s.RT < rows) {
-      float f[V];
-      v[i].get(f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[PC == 1 ? 0 : j] += f[j];
-    }
-  }
-  s.sum(acc, part, stat);
-  s.mine(stat, mu);
-#pragma unroll
-  for (int p = 0; p < PC; ++p) {
-    mu[p] /= count;
-    acc[p] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (s.on && s.rt + i * s.RT < rows) {
-      float f[V];
-      v[i].get(f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = j < s.n ? f[j] - mu[PC == 1 ? 0 : j] : 0.f;
-        acc[PC == 1 ? 0 : j] += d * d;
-      }
-    }
-  }
-  s.sum(acc, part, stat + kMaxGroups);
+    for (int j = 0; j < V; ++j) u[j] = act.run<KIND>((u[j] - f.mu[PC == 1 ? 0 : j]) * f.scale[j] + f.shift[j]);
+    Vec16<T> w;
+    w.set(u);
+    w.store(y + i * step);
+  });
+}
+template <class T, int NT, int R, int RL, int PC>
+__device__ __forceinline__ void write(Held<T, NT, R, RL>& h, const Affine<T, PC>& f, int act, int count, char* lds, T* y,
+                                      int64_t step) {
+  if (act <= DML_ACT_RELU) write_as<kClamp>(h, f, act_parameters(act), count, lds, y, step);
+  else if (act == DML_ACT_GELU) write_as<kErf>(h, f, act_parameters(act), count, lds, y, step);
+  else write_as<kSwish>(h, f, act_parameters(act), count, lds, y, step);
 }
 
-template <class T, int NT, int R, bool CH>
+template <class T, int NT, int R, int RL, bool ONCE, bool CH>
 __global__ __launch_bounds__(NT) void one_pass(DmlGroupNormArgs a, int S) {
   typedef Slab<T, NT, CH> SL;
   constexpr int V = SL::V, PC = SL::PC;
-  __shared__ __attribute__((aligned(16))) float part[NT * PC];
+  __shared__ float2 part[NT * PC];
   __shared__ float stat[2 * kMaxGroups];
+  __shared__ __attribute__((aligned(16))) char lds[RL > 0 ? RL * NT * 16 : 16];
   const int slabs = a.C / S, b = xcd_remap(blockIdx.x, gridDim.x);  // a sample's slabs share DRAM pages and lines
   const int n = b / slabs, c0 = (b - n * slabs) * S;
   const SL s(S, a.C / a.G);
-  const int c = c0 + s.col * V;
-  Vec16<T> v[R];
+  const int c = c0 + s.c, count = s.on ? s.rows_of(s.rt, a.HW) : 0;
+  Held<T, NT, R, RL> h;
   Affine<T, PC> f;
-  const float count = (float)a.HW * (float)s.cg;
-  read_and_sum<T, NT, R, CH>(s, (const T*)a.x + n * a.xn + c, a.ldx, a.HW, count, v, f.mu, part, stat);
+  read_and_sum<T, NT, R, RL, ONCE, CH>(s, (const T*)a.x + n * a.xn + c, a.ldx, a.HW, h, count, lds, part, stat,
+                                 [&] { f.load(a, c); });
   if (!s.on) return;
-  f.load(a, c, s.n);
+  s.mine(stat, f.mu);
   float var[PC];
   s.mine(stat + kMaxGroups, var);
+  const float inv = 1.f / ((float)a.HW * (float)s.cg);
 #pragma unroll
-  for (int j = 0; j < V; ++j) f.scale[j] *= 1.f / sqrtf(var[PC == 1 ? 0 : j] / count + a.eps);
-  T* y = (T*)a.y + n * a.yn + c;
+  for (int p = 0; p < PC; ++p) var[p] = __builtin_amdgcn_rsqf(var[p] * inv + a.eps);
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int r = s.rt + i * s.RT;
-    if (r < a.HW) {
-      f.apply(v[i], a.act);
-      s.store(v[i], y + (int64_t)r * a.ldy);
-    }
-  }
+  for (int j = 0; j < V; ++j) f.scale[j] *= var[PC == 1 ? 0 : j];
+  T* y = (T*)a.y + n * a.yn + c + s.rt * a.ldy;
+  const int64_t step = s.RT * a.ldy;
+  write(h, f, a.act, count, lds, y, step);
 }
 
 // (mean, M2) of each group over one chunk of rows -> ws[(n G + g) chunks + chunk]
 template <class T, int NT, int R, bool CH>
 __global__ __launch_bounds__(NT) void stats(DmlGroupNormArgs a, int S, int rows, int chunks) {
   typedef Slab<T, NT, CH> SL;
-  __shared__ __attribute__((aligned(16))) float part[NT * SL::PC];
+  __shared__ float2 part[NT * SL::PC];
   __shared__ float stat[2 * kMaxGroups];
   const int slabs = a.C / S;
   int b = xcd_remap(blockIdx.x, gridDim.x);
   const int slab = b % slabs, chunk = (b /= slabs) % chunks, n = b / chunks;
   const SL s(S, a.C / a.G);
   const int row0 = chunk * rows, mine = min(rows, a.HW - row0);
-  Vec16<T> v[R];
-  float mu[SL::PC];
-  const float count = (float)mine * (float)s.cg;
-  read_and_sum<T, NT, R, CH>(s, (const T*)a.x + n * a.xn + row0 * a.ldx + slab * S + s.col * SL::V, a.ldx, mine, count,
-                             v, mu, part, stat);
+  Held<T, NT, R, 0> h;
+  read_and_sum<T, NT, R, 0, false, CH>(s, (const T*)a.x + n * a.xn + row0 * a.ldx + slab * S + s.c, a.ldx, mine, h,
+                                s.on ? s.rows_of(s.rt, mine) : 0, nullptr, part, stat, [] {});
   for (int g = threadIdx.x; g < s.gs; g += NT)
-    ((float2*)a.ws)[((int64_t)n * a.G + slab * s.gs + g) * chunks + chunk] =
-        make_float2(stat[g] / count, stat[kMaxGroups + g]);
+    ((float2*)a.ws)[((int64_t)n * a.G + slab * s.gs + g) * chunks + chunk] = make_float2(stat[g], stat[kMaxGroups + g]);
 }
 
 template <class T, int NT, int R, bool CH>
@@ -225,17 +279,16 @@ __global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows,
       stat[kMaxGroups + g] = 1.f / sqrtf(m2 / total + a.eps);
     }
   }
-  const int c = slab * S + s.col * V, row0 = chunk * rows, mine = min(rows, a.HW - row0);
+  const int c = slab * S + s.c, row0 = chunk * rows, mine = min(rows, a.HW - row0);
   const T* x = (const T*)a.x + n * a.xn + row0 * a.ldx + c;
   T* y = (T*)a.y + n * a.yn + row0 * a.ldy + c;
-  Vec16<T> v[R];
+  const int count = s.on ? s.rows_of(s.rt, mine) : 0;
+  Held<T, NT, R, 0> h;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int r = s.rt + i * s.RT;
-    if (s.on && r < mine) s.load(v[i], x + (int64_t)r * a.ldx);
-  }
+  for (int i = 0; i < R; ++i)
+    if (i < count) h.v[i].load(x + (int64_t)(s.rt + i * s.RT) * a.ldx);
   Affine<T, PC> f;
-  f.load(a, c, s.on ? s.n : 0);
+  f.load(a, c);
   __syncthreads();
   if (!s.on) return;
   s.mine(stat, f.mu);
@@ -243,19 +296,13 @@ __global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows,
   s.mine(stat + kMaxGroups, rs);
 #pragma unroll
   for (int j = 0; j < V; ++j) f.scale[j] *= rs[PC == 1 ? 0 : j];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int r = s.rt + i * s.RT;
-    if (r < mine) {
-      f.apply(v[i], a.act);
-      s.store(v[i], y + (int64_t)r * a.ldy);
-    }
-  }
+  write(h, f, a.act, count, nullptr, y + s.rt * a.ldy, s.RT * a.ldy);
 }
 
-// Groups wider than 1024 vectors: a workgroup per (sample, group), three reads.
+// What no slab fits: groups wider than 1024 vectors, fewer channels than a vector has. A workgroup per
+// (sample, group), element by element, three reads.
 template <class T>
-__global__ __launch_bounds__(256) void wide_groups(DmlGroupNormArgs a) {
+__global__ __launch_bounds__(256) void by_element(DmlGroupNormArgs a) {
   __shared__ float part[4];
   const int g = blockIdx.x % a.G, n = blockIdx.x / a.G;
   const int cg = a.C / a.G, c0 = g * cg;
@@ -282,87 +329,105 @@ __global__ __launch_bounds__(256) void wide_groups(DmlGroupNormArgs a) {
   const float rs = 1.f / sqrtf(total(s) / (float)count + a.eps);
   for (int64_t i = threadIdx.x; i < count; i += 256) {
     const int c = (int)(i % cg);
-    float v[1] = {(to_f32(x[(i / cg) * a.ldx + c]) - mu) * (rs * (a.weight ? a.weight[c0 + c] : 1.f)) +
-                  (a.bias ? a.bias[c0 + c] : 0.f)};
-    activate(v, a.act);
-    y[(i / cg) * a.ldy + c] = (T)v[0];
+    const float v = (to_f32(x[(i / cg) * a.ldx + c]) - mu) * (rs * (a.weight ? a.weight[c0 + c] : 1.f)) +
+                    (a.bias ? a.bias[c0 + c] : 0.f);
+    y[(i / cg) * a.ldy + c] = (T)activate(v, a.act);
   }
 }
 
-// The plan of a call: mode 0 = one pass, 1 = statistics and application apart, 2 = wide groups.
+// How a call runs: slabs of S channels through one_pass (a row of kShapes), through stats + apply, or element
+// by element.
+enum { ONE_PASS, SPLIT, ELEMENTS };
 struct Plan {
-  int mode, S, NT, R, rows, chunks;
+  int mode, S, shape, rows, chunks;
   bool ch;
 };
 
+// one_pass forms: threads, vectors in registers and in LDS, loads marked as not read again. 14 vectors a thread leave
+// two 512-thread or four 256-thread workgroups on a CU, and long slabs beat many short ones (256 x 49 x 2048 bf16,
+// 256 threads: 23.1 us at 14 vectors, 29.8 at 7, 42 at 4), so a thread holds 14 where there is that much. The last form
+// fills a CU with one workgroup: 400 KiB, for 128-byte runs where the slab is long (256 x 3136 x 256 bf16: 180 us,
+// against 190 with half the run). It copies into LDS directly, which takes 16-byte alignment. The mark gave the large
+// cases 5 to 12 % where a pixel's run is half a cache line or more (256 x 784 x 512 bf16: 92 -> 82 us) and cost 15 %
+// where it is 32 bytes.
+constexpr int kShapes[][4] = {{256, 2, 0, 0},  {256, 6, 0, 0},   {256, 14, 0, 1}, {512, 14, 0, 0},
+                              {512, 14, 0, 1}, {1024, 16, 0, 1}, {1024, 16, 9, 1}};
+
 static Plan plan(const DmlGroupNormArgs* a) {
   const int es = a->dtype == DML_F32 ? 4 : 2, V = 16 / es, cg = a->C / a->G;
+  const bool aligned = (((uintptr_t)a->x | (uintptr_t)(a->xn * es) | (uintptr_t)(a->ldx * es)) & 15) == 0;
+  const double bytes = 2.0 * es * a->N * a->HW * a->C;
   Plan p = {};
   p.ch = cg % V != 0;
-  if ((cg + V - 1) / V > 1024) {
-    p.mode = 2;
-    return p;
-  }
-  // A slab is a number of groups that divides G, best with whole vectors (partial ones at a slab's
-  // end are loaded by the element). Wanted: runs of 128 bytes (a cache line) a pixel; a slab that
-  // fits the registers of a workgroup; 512 workgroups, so that some load while others store.
-  auto cost = [&](int k, bool fit_only) -> long {
+  const double ops = (p.ch ? 16 : 12) + (a->act == DML_ACT_GELU ? 22 : a->act >= DML_ACT_SILU ? 14 : 2);
+  double best = 1e30;
+  // Estimated microseconds of each slab width, from measurements: memory at 5300 bytes/ns for runs of 128 bytes a
+  // pixel, less for shorter ones (they cost lines); a lone CU's 60 bytes/ns, by the same rule, and
+  // `ops` instructions a value on its 64 lanes; 4.4 ns a workgroup.
+  // stats + apply read twice (the second time partly from cache) and pay a second launch.
+  for (int k = 1; k <= a->G && k <= kMaxGroups; ++k) {
     const long S = (long)k * cg, cols = (S + V - 1) / V;
-    if (cols > 1024) return -1;
-    const long cap = (1024 / cols) * 16;  // rows that one_pass<1024, 16> holds
-    if (fit_only && a->HW > cap) return -1;
-    const long wgs = (long)a->N * (a->C / S);
-    long c = 0;
-    if (S % V) c += 400;                       // element loads
-    if (S * es < 128) c += (128 - S * es) * 2;  // short runs
-    if (wgs < 512) c += (512 - wgs);
-    c += S * es / 64;                           // else the narrower
-    return c;
-  };
-  int best = 0;
-  long bc = 0;
-  for (int fit = 1; fit >= 0 && !best; --fit)
-    for (int k = 1; k <= a->G && k <= kMaxGroups; ++k) {
-      if (a->G % k) continue;
-      const long c = cost(k, fit);
-      if (c >= 0 && (!best || c < bc)) best = k, bc = c;
+    if (a->G % k || S < V || cols > 1024) continue;
+    const double run = (double)(S * es), eff = run >= 128 ? 1.0 : run / (run + 24);
+    const double wgs = (double)a->N * (a->C / S), slab = 2 * run * a->HW;
+    const double stream = bytes / 5.3e6 / eff, r = (run < 128 ? run / 128 : 1.0) * 60e3;
+    for (int i = 0; i < (int)(sizeof(kShapes) / sizeof(kShapes[0])); ++i) {
+      const int* f = kShapes[i];
+      if (f[2] ? p.ch || !aligned || run < 64 : f[1] == 14 && f[3] != (run >= 64)) continue;
+      if (cols > f[0] || a->HW > f[0] / cols * (f[1] + f[2])) continue;
+      const double rounds = (double)(long)((wgs + 255) / 256);
+      const double own = 3 + rounds * slab * (1 / r + ops / (2 * es * 64 * 2100.0));
+      const double t = (own > stream ? own : stream) + 4.4e-3 * wgs;
+      if (t < best) {
+        best = t;
+        p.mode = ONE_PASS, p.S = (int)S, p.shape = i;
+      }
+      break;  // the smallest form that holds the slab
     }
-  p.S = best * cg;
-  const int cols = (p.S + V - 1) / V;
-  const long wgs = (long)a->N * (a->C / p.S), slab = (long)a->HW * p.S * es;
-  const int RT256 = 256 / cols, RT = 1024 / cols;
-  if (cols <= 256 && a->HW <= (long)RT256 * 8) {
-    p.NT = 256;
-    p.R = a->HW <= RT256 * 2 ? 2 : 8;
-    return p;
+    const double t = 1.55 * stream + 8;
+    if (t < best) {
+      best = t;
+      p.mode = SPLIT, p.S = (int)S;
+      const int RT = (int)(256 / cols);
+      // 8 rows a thread, 4 where that leaves CUs idle; more threads where the rows are wide
+      p.shape = cols > 256 ? 2 : wgs * ((a->HW + RT * 8 - 1) / (RT * 8)) < 1024;
+      p.rows = p.shape == 2 ? (int)(1024 / cols) * 4 : RT * (p.shape ? 4 : 8);
+      p.chunks = (a->HW + p.rows - 1) / p.rows;
+    }
   }
-  p.NT = 1024;
-  if (a->HW <= (long)RT * 16 && !(wgs < 128 && slab > 128 * 1024)) {
-    p.R = a->HW <= RT * 4 ? 4 : a->HW <= RT * 8 ? 8 : 16;
-    return p;
-  }
-  p.mode = 1;
-  p.R = 4;
-  p.rows = RT * p.R;
-  p.chunks = (a->HW + p.rows - 1) / p.rows;
+  if (best == 1e30) p.mode = ELEMENTS;
   return p;
+}
+
+template <class T, int I, bool CH>
+static void launch_one(const DmlGroupNormArgs* a, const Plan& p, dim3 grid, hipStream_t s) {
+  if constexpr (!(CH && kShapes[I][2])) {
+    if (p.shape == I)
+      hipLaunchKernelGGL((one_pass<T, kShapes[I][0], kShapes[I][1], kShapes[I][2], kShapes[I][3], CH>), grid, dim3(kShapes[I][0]), 0,
+                         s, *a, p.S);
+  }
+  if constexpr (I > 0) launch_one<T, I - 1, CH>(a, p, grid, s);
+}
+
+template <class T, int NT, int R, bool CH>
+static void launch_split(const DmlGroupNormArgs* a, const Plan& p, dim3 grid, hipStream_t s) {
+  hipLaunchKernelGGL((stats<T, NT, R, CH>), grid, dim3(NT), 0, s, *a, p.S, p.rows, p.chunks);
+  hipLaunchKernelGGL((apply<T, NT, R, CH>), grid, dim3(NT), 0, s, *a, p.S, p.rows, p.chunks);
 }
 
 template <class T, bool CH>
 static int launch(const DmlGroupNormArgs* a, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)((long)a->N * (p.mode == 2 ? a->G : a->C / p.S) * (p.mode == 1 ? p.chunks : 1)));
-  if (p.mode == 2) {
-    hipLaunchKernelGGL(wide_groups<T>, grid, dim3(256), 0, s, *a);
-  } else if (p.mode == 1) {
-    hipLaunchKernelGGL((stats<T, 1024, 4, CH>), grid, dim3(1024), 0, s, *a, p.S, p.rows, p.chunks);
-    hipLaunchKernelGGL((apply<T, 1024, 4, CH>), grid, dim3(1024), 0, s, *a, p.S, p.rows, p.chunks);
-  } else if (p.NT == 256) {
-    if (p.R == 2) hipLaunchKernelGGL((one_pass<T, 256, 2, CH>), grid, dim3(256), 0, s, *a, p.S);
-    else hipLaunchKernelGGL((one_pass<T, 256, 8, CH>), grid, dim3(256), 0, s, *a, p.S);
+  const dim3 grid((unsigned)((long)a->N * (p.mode == ELEMENTS ? a->G : a->C / p.S) * (p.mode == SPLIT ? p.chunks : 1)));
+  if (p.mode == ELEMENTS) {
+    hipLaunchKernelGGL(by_element<T>, grid, dim3(256), 0, s, *a);
+  } else if (p.mode == ONE_PASS) {
+    launch_one<T, sizeof(kShapes) / sizeof(kShapes[0]) - 1, CH>(a, p, grid, s);
+  } else if (p.shape == 0) {
+    launch_split<T, 256, 8, CH>(a, p, grid, s);
+  } else if (p.shape == 1) {
+    launch_split<T, 256, 4, CH>(a, p, grid, s);
   } else {
-    if (p.R == 4) hipLaunchKernelGGL((one_pass<T, 1024, 4, CH>), grid, dim3(1024), 0, s, *a, p.S);
-    else if (p.R == 8) hipLaunchKernelGGL((one_pass<T, 1024, 8, CH>), grid, dim3(1024), 0, s, *a, p.S);
-    else hipLaunchKernelGGL((one_pass<T, 1024, 16, CH>), grid, dim3(1024), 0, s, *a, p.S);
+    launch_split<T, 1024, 4, CH>(a, p, grid, s);
   }
   DML_CHECK_LAUNCH();
   return 0;
@@ -387,28 +452,18 @@ static int check(const DmlGroupNormArgs* a) {
 }  // namespace gn
 }  // namespace dml
 
-extern "C" int64_t dml_group_norm_workspace(const DmlGroupNormArgs* a) {
+extern "C" int64_t dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s) {
   using namespace dml::gn;
   if (check(a) != 0) return -1;
   if (a->N == 0 || a->HW == 0) return 0;
   const Plan p = plan(a);
-  return p.mode == 1 ? (int64_t)a->N * a->G * p.chunks * 8 : 0;
-}
-
-extern "C" int dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s) {
-  using namespace dml::gn;
-  if (check(a) != 0) return -1;
-  if (a->N == 0 || a->HW == 0) return 0;
-  const Plan p = plan(a);
-  const long per = (long)a->N * (p.mode == 2 ? a->G : a->C / p.S);
-  if (per > 0x7fffffffl || (p.mode == 1 && per > 0x7fffffffl / p.chunks)) {
+  const long per = (long)a->N * (p.mode == ELEMENTS ? a->G : a->C / p.S);
+  if (per > 0x7fffffffl || (p.mode == SPLIT && per > 0x7fffffffl / p.chunks)) {
     dml_set_error("dml_group_norm: over 2^31 workgroups");
     return -1;
   }
-  if (p.mode == 1 && (!a->ws || a->ws_bytes < (int64_t)a->N * a->G * p.chunks * 8)) {
-    dml_set_error("dml_group_norm: workspace missing or smaller than dml_group_norm_workspace says");
-    return -1;
-  }
+  const int64_t need = p.mode == SPLIT ? (int64_t)a->N * a->G * p.chunks * 8 : 0;
+  if (need > a->ws_bytes || (need && !a->ws)) return need;
   switch (a->dtype) {
     case DML_BF16: return p.ch ? launch<bf16, true>(a, p, s) : launch<bf16, false>(a, p, s);
     case DML_F16: return p.ch ? launch<dml::f16, true>(a, p, s) : launch<dml::f16, false>(a, p, s);

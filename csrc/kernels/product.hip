@@ -85,9 +85,9 @@ __device__ __forceinline__ void finish(const DmlProductArgs& a, int e, int row, 
   float r = 0.f;
   if (a.res)
     r = a.out_f32 ? ((const float*)a.res)[row * a.ldr + col] : to_f32(((const T*)a.res)[row * a.ldr + col]);
-  float f[1] = {a.act_last ? v + r : v};
-  activate(f, a.act);
-  v = a.act_last ? f[0] : f[0] + r;
+  if (a.act_last) v += r;
+  v = activate(v, a.act);
+  if (!a.act_last) v += r;
   if (a.out_f32) ((float*)a.y)[row * a.ldy + col] = v;
   else ((T*)a.y)[row * a.ldy + col] = (T)v;
 }

@@ -8,6 +8,7 @@ or ValueError before anything is launched, a failure of the library raises ``Nat
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -29,6 +30,8 @@ def _act(act: str) -> int:
 def _pitch(t: torch.Tensor, first: int, what: str) -> Tuple[int, int]:
     """(rows, elements from one row to the next) of dimensions first .. -2 of t seen as rows of its last one."""
     shape, stride = t.shape, t.stride()
+    if t.is_contiguous():
+        return math.prod(shape[first:-1]), shape[-1]
     if shape[-1] > 1 and stride[-1] != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous, got strides {stride}")
     rows, pitch = 1, None
@@ -93,12 +96,20 @@ def _ready(*tensors: Optional[torch.Tensor]) -> None:
         raise ValueError(f"expected tensors on a HIP device, got {dev}")
 
 
-def _launch(fn, args, device: torch.device, what: str) -> None:
-    if device.index == torch.cuda.current_device():
-        N.check(fn(C.byref(args), N.stream_ptr()), what)
+def _launch(fn, a, device: torch.device, what: str) -> int:
+    """fn(a, the current stream of device), with device current."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        rc = fn(C.byref(a), torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(device):
-            N.check(fn(C.byref(args), N.stream_ptr()), what)
+        with torch.cuda.device(i):
+            rc = fn(C.byref(a), torch._C._cuda_getCurrentRawStream(i))
+    return N.check(rc, what) if rc else 0
+
+
+def _f32(v: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """v as contiguous fp32; v itself where it is that."""
+    return v if v is None or v.dtype is torch.float32 and v.is_contiguous() else v.float().contiguous()
 
 
 def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = None,
@@ -142,18 +153,16 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     if not out.numel():
         return out
-    if weight is not None:
-        weight = weight.float().contiguous()
-    if bias is not None:
-        bias = bias.float().contiguous()
+    weight, bias = _f32(weight), _f32(bias)
     a = N.GroupNormArgs(x.data_ptr(), out.data_ptr(), weight.data_ptr() if weight is not None else None,
                         bias.data_ptr() if bias is not None else None, x.stride(0), out.stride(0),
                         ldx, ldy, None, 0, n, rows, c, groups, _DTYPES[x.dtype], code, eps)
-    a.ws_bytes = N.check(N.lib().dml_group_norm_workspace(C.byref(a)), "dml_group_norm_workspace")
-    if a.ws_bytes:
-        ws = torch.empty(a.ws_bytes, device=x.device, dtype=torch.uint8)
-        a.ws = ws.data_ptr()
-    _launch(N.lib().dml_group_norm, a, x.device, "dml_group_norm")
+    fn = N.lib().dml_group_norm
+    need = _launch(fn, a, x.device, "dml_group_norm")
+    if need:
+        ws = torch.empty(need, device=x.device, dtype=torch.uint8)
+        a.ws, a.ws_bytes = ws.data_ptr(), need
+        _launch(fn, a, x.device, "dml_group_norm")
     return out
 
 
@@ -206,8 +215,7 @@ def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, wha
         return out
     if e == 0:
         return out.zero_() if fill else out
-    if bias is not None:
-        bias = bias.float().contiguous()
+    bias = _f32(bias)
     a = N.ProductArgs(x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
                       residual.data_ptr() if residual is not None else None, out.data_ptr(),
                       ends.data_ptr() if ends is not None else None, ldx, ldw,
