@@ -8,10 +8,14 @@
 // The ends are read on the device and clamped to an ascending sequence within [0, M], so no
 // content of theirs reaches past a tensor.
 #include "activation.h"
+#include "conv_shared.h"
 #include <climits>
 
 namespace dml {
 namespace prod {
+
+using convk::lds_void;
+using convk::wait_vmcnt;
 
 // Where a row tile lies: group e, rows [row, row + rows) of the tensors; rows = 0: none.
 struct Place {
@@ -55,8 +59,8 @@ __device__ __forceinline__ Place locate(const DmlProductArgs& a, int t) {
     if (past) {
       const int l = __builtin_ctzll(past);
       const int first = __shfl(upto - tiles, l, 64), b = __shfl(beg, l, 64), n = __shfl(end, l, 64);
-      const int row = b + (t - first) * BM;
-      return {base + l, row, min(BM, n - row)};
+      const int row = __builtin_amdgcn_readfirstlane(b + (t - first) * BM);
+      return {__builtin_amdgcn_readfirstlane(base + l), row, __builtin_amdgcn_readfirstlane(min(BM, n - row))};
     }
     start = __shfl(end, 63, 64);
     before = __shfl(upto, 63, 64);
@@ -78,74 +82,296 @@ template <> struct Mfma<f16> {
   }
 };
 
-// One output element: row `row`, column `col` of group e.
-template <class T>
-__device__ __forceinline__ void finish(const DmlProductArgs& a, int e, int row, int col, float v) {
-  if (a.bias) v += a.bias[e * a.bias_group + col];
-  float r = 0.f;
-  if (a.res)
-    r = a.out_f32 ? ((const float*)a.res)[row * a.ldr + col] : to_f32(((const T*)a.res)[row * a.ldr + col]);
-  if (a.act_last) v += r;
-  v = activate(v, a.act);
-  if (!a.act_last) v += r;
-  if (a.out_f32) ((float*)a.y)[row * a.ldy + col] = v;
-  else ((T*)a.y)[row * a.ldy + col] = (T)v;
+// Eight columns from `col` of one row through the epilogue; `n` of them exist.
+template <int KIND, class T>
+__device__ __forceinline__ void finish8(const DmlProductArgs& a, Act act, int64_t row, int col, int n, float (&v)[8],
+                                        const float (&bias)[8]) {
+  float r[8] = {};
+  if (a.res) {
+    if (a.out_f32) {
+      const float* p = (const float*)a.res + row * a.ldr + col;
+      if (n >= 8) __builtin_memcpy(r, p, 32);
+      else
+        for (int j = 0; j < 8; ++j)
+          if (j < n) r[j] = p[j];
+    } else {
+      const T* p = (const T*)a.res + row * a.ldr + col;
+      T t[8] = {};
+      if (n >= 8) __builtin_memcpy(t, p, 16);
+      else
+        for (int j = 0; j < 8; ++j)
+          if (j < n) t[j] = p[j];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = to_f32(t[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] += bias[j];
+  if (a.act_last) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act.run<KIND>(v[j] + r[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = act.run<KIND>(v[j]) + r[j];
+  }
+  if (a.out_f32) {
+    float* p = (float*)a.y + row * a.ldy + col;
+    if (n >= 8) __builtin_memcpy(p, v, 32);
+    else
+      for (int j = 0; j < 8; ++j)
+        if (j < n) p[j] = v[j];
+  } else {
+    T* p = (T*)a.y + row * a.ldy + col;
+    T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = (T)v[j];
+    if (n >= 8) __builtin_memcpy(p, t, 16);
+    else
+      for (int j = 0; j < 8; ++j)
+        if (j < n) p[j] = t[j];
+  }
 }
 
-// Tiles of 64 x 64, four waves of 32 x 32, operands through LDS 32 deep; any K, strides and
-// alignment (elements are loaded one by one).
-template <class T>
-__global__ __launch_bounds__(256) void product_simple(DmlProductArgs a) {
-  typedef typename Mfma<T>::vec vec;
-  constexpr int BM = 64, BN = 64, P = 40;  // LDS row pitch in elements
-  __shared__ __attribute__((aligned(16))) T sx[BM * P], sw[BN * P];
-  const int ntn = (a.N + BN - 1) / BN;
-  const Place at = locate<BM>(a, blockIdx.x / ntn);
-  if (at.rows <= 0) return;
-  const int n0 = (blockIdx.x % ntn) * BN;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const bool fill = at.e >= a.E;
-  const T* x = (const T*)a.x + at.row * a.ldx;
-  const T* w = (const T*)a.w + (fill ? 0 : at.e) * a.w_group + n0 * a.ldw;
-  f32x4 acc[2][2] = {};
-  const int wm = (wid >> 1) * 32, wn = (wid & 1) * 32;
-  const int r = tid >> 2, kc = (tid & 3) * 8;
-  for (int k0 = 0; k0 < (fill ? 0 : a.K); k0 += 32) {
+// A wave's accumulators (rows wm.., columns col0..) through the epilogue.
+template <int KIND, class C>
+__device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
+                                          int col0, int lane) {
+  const Act act = act_parameters(a.act);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = k0 + kc + j;
-      sx[r * P + kc + j] = r < at.rows && k < a.K ? x[r * a.ldx + k] : (T)0.f;
-      sw[r * P + kc + j] = n0 + r < a.N && k < a.K ? w[r * a.ldw + k] : (T)0.f;
-    }
-    __syncthreads();
-    vec fx[2], fw[2];
+  for (int p = 0; p < C::FI / 2; ++p) {
+    const int col = col0 + p * 32 + (lane >> 4) * 8, n = a.N - col;
+    float bias[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fx[i] = *(const vec*)(sx + (wm + i * 16 + (lane & 15)) * P + (lane >> 4) * 8);
-      fw[i] = *(const vec*)(sw + (wn + i * 16 + (lane & 15)) * P + (lane >> 4) * 8);
-    }
+    for (int j = 0; j < 8; ++j) bias[j] = a.bias && j < n ? a.bias[at.e * a.bias_group + col + j] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = Mfma<T>::run(fw[i], fx[j], acc[i][j]);
-    __syncthreads();
-  }
-  // lane: columns 4 (lane >> 4) + q of weight fragment i, row lane & 15 of row fragment j
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < C::FJ; ++j) {
+      const int m = wm + j * 16 + (lane & 15);
+      float v[8];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int m = wm + j * 16 + (lane & 15), col = n0 + wn + i * 16 + (lane >> 4) * 4 + q;
-        if (m >= at.rows || col >= a.N) continue;
-        if (fill) {
-          if (a.out_f32) ((float*)a.y)[(at.row + m) * a.ldy + col] = 0.f;
-          else ((T*)a.y)[(at.row + m) * a.ldy + col] = (T)0.f;
-        } else {
-          finish<T>(a, at.e, at.row + m, col, acc[i][j][q]);
-        }
+        v[q] = acc[2 * p][j][q];
+        v[4 + q] = acc[2 * p + 1][j][q];
       }
+      if (m < at.rows && n > 0) finish8<KIND, typename C::T>(a, act, (int64_t)at.row + m, col, n, v, bias);
+    }
+  }
+}
+
+template <class C>
+__device__ __forceinline__ void finish(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
+                                       int col0, int lane) {
+  if (a.act <= DML_ACT_RELU) finish_as<kClamp, C>(a, at, acc, wm, col0, lane);
+  else if (a.act == DML_ACT_GELU) finish_as<kErf, C>(a, at, acc, wm, col0, lane);
+  else finish_as<kSwish, C>(a, at, acc, wm, col0, lane);
+}
+
+// Zeros into rows wm .. wm + rows, columns col0 .. col0 + cols of a tile.
+template <class T>
+__device__ __forceinline__ void zero_rows(const DmlProductArgs& a, const Place& at, int col0, int cols, int wm, int rows,
+                                          int lane) {
+  for (int m = wm; m < min(wm + rows, at.rows); ++m)
+    for (int c = col0 + lane; c < min(col0 + cols, a.N); c += 64) {
+      const int64_t i = (int64_t)(at.row + m) * a.ldy + c;
+      if (a.out_f32) ((float*)a.y)[i] = 0.f;
+      else ((T*)a.y)[i] = (T)0.f;
+    }
+}
+
+// ---- tiles through LDS ----
+//
+// A workgroup of WM x WN waves computes BM rows x BN columns, D[column][row] = W X^T: the MFMA rows are output columns,
+// so a lane holds runs of columns of one row. Operands go through LDS in K slices of 64 (whole 128-byte lines of a
+// row; slices of 32 had the L2 serve twice the requests: 8192^3 bf16 904 us against 824), two slices in turn, copied
+// there by LDS-DMA. The fragments of one half slice are read while the other's products run: a row fragment's
+// register is refilled as soon as its products are issued, the column fragments alternate. So a wave waits once a
+// slice, at the barrier that hands over the next one, and the slice behind that is requested right after it.
+//
+// 16-byte chunks lie in a tile row XORed with a key of the row, chosen so that the lanes that LDS serves together
+// (0-3, 12-15, 20-23, 24-27 and so on) hit all 64 banks with both operands' row patterns: no conflicts by the counters.
+template <class T_, int BM_, int BN_, int WM_, int WN_, bool DMA_>
+struct Tile {
+  typedef T_ T;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = 64;
+  static constexpr bool DMA = DMA_;
+  static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int TM = BM / WM, TN = BN / WN;            // rows, columns of a wave
+  static constexpr int FJ = TM / 16, FI = TN / 16;            // fragments along rows, columns
+  static constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW;    // pieces of 8 tile rows that a wave copies per slice
+  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
+  static constexpr int MINW = (LDS <= 40960 ? 4 : LDS <= 81920 ? 2 : 1) * NW / 4;  // waves a SIMD that LDS leaves room for
+  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && TN % 32 == 0 && TM % 16 == 0 && LDS <= 163840, "tile");
+  __device__ __forceinline__ static int xkey(int row) { return row & 7; }
+  __device__ __forceinline__ static int wkey(int row) { return (row & 3) | ((row >> 1) & 4); }
+};
+
+// Without DMA (operands that are not 16-byte aligned, or rows too far apart for its 32-bit offsets): the same copies
+// through registers, loaded half a slice ahead of the barrier that frees their place.
+template <class C>
+__global__ __launch_bounds__(C::NT, C::MINW) void product_tile(DmlProductArgs a) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host needs the entry only
+  typedef typename C::T T;
+  typedef typename Mfma<T>::vec vec;
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+  // blocks of one XCD take neighbouring tiles, eight row tiles by all column tiles at a time
+  const int ntn = (a.N + C::BN - 1) / C::BN, nb = gridDim.x;
+  const int b = xcd_remap(blockIdx.x, nb), s0 = b / (8 * ntn) * 8;
+  const int high = min(8, nb / ntn - s0), r = b - s0 * ntn;
+  const int tn = r / high, tm = s0 + r - tn * high;
+  const Place at = locate<C::BM>(a, tm);
+  if (at.rows <= 0) return;
+  const int n0 = tn * C::BN, cols = a.N - n0;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wid / C::WN * C::TM, wn = wid % C::WN * C::TN;
+  if (at.e >= a.E) {
+    zero_rows<T>(a, at, n0 + wn, C::TN, wm, C::TM, lane);
+    return;
+  }
+  const int nk = (a.K + C::BK - 1) / C::BK;
+  const T* const x = (const T*)a.x + at.row * a.ldx;
+  const T* const w = (const T*)a.w + at.e * a.w_group + (int64_t)n0 * a.ldw;
+
+  // A copy piece is 8 tile rows: lane l fills place l % 8 of row l / 8, so it fetches the chunk that belongs there.
+  // With DMA, rows and chunks outside the operands get an offset past the descriptor's range: it writes zeros.
+  const int lrow = lane >> 3, lplace = lane & 7;
+  const int xrow0 = wid * C::XI * 8 + lrow, wrow0 = wid * C::WI * 8 + lrow;
+  const int dx = wid * C::XI * 1024, dw = C::BM * 128 + wid * C::WI * 1024;
+  constexpr unsigned kOut = 0x80000000u;
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)x, 0, 0x7ffffff0, 0x00020000);
+  const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)w, 0, 0x7ffffff0, 0x00020000);
+  unsigned ox[C::XI], ow[C::WI];
+  uint4 hx[C::DMA ? 1 : C::XI], hw[C::DMA ? 1 : C::WI];
+  if constexpr (C::DMA) {
+#pragma unroll
+    for (int j = 0; j < C::XI; ++j) {
+      const int row = xrow0 + j * 8;
+      ox[j] = row < at.rows ? (unsigned)(row * (int)(a.ldx * 2) + (lplace ^ C::xkey(row)) * 16) : kOut;
+    }
+#pragma unroll
+    for (int j = 0; j < C::WI; ++j) {
+      const int row = wrow0 + j * 8;
+      ow[j] = row < cols ? (unsigned)(row * (int)(a.ldw * 2) + (lplace ^ C::wkey(row)) * 16) : kOut;
+    }
+  }
+  auto fetch = [&](uint4& v, const T* p, int k) {  // the eight values from k of a row; 0 behind K
+    if (k + 8 <= a.K) {
+      __builtin_memcpy(&v, p + k, 16);
+    } else {
+      T t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = k + i < a.K ? p[k + i] : (T)0.f;
+      __builtin_memcpy(&v, t, 16);
+    }
+  };
+  // request slice kt: by DMA into `stage`, or into hx and hw
+  auto issue = [&](int kt, int stage) {
+    const int k0 = kt * C::BK;
+    if constexpr (C::DMA) {
+      if (k0 + C::BK > a.K) {  // chunks past K are out from now on
+#pragma unroll
+        for (int j = 0; j < C::XI; ++j)
+          if (k0 + (lplace ^ C::xkey(xrow0 + j * 8)) * 8 >= a.K) ox[j] = kOut;
+#pragma unroll
+        for (int j = 0; j < C::WI; ++j)
+          if (k0 + (lplace ^ C::wkey(wrow0 + j * 8)) * 8 >= a.K) ow[j] = kOut;
+      }
+#pragma unroll
+      for (int j = 0; j < C::XI; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(smem + dx + stage * C::STAGE + j * 1024), 16, ox[j],
+                                                 k0 * 2, 0, 0);
+#pragma unroll
+      for (int j = 0; j < C::WI; ++j)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(smem + dw + stage * C::STAGE + j * 1024), 16, ow[j],
+                                                 k0 * 2, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C::XI; ++j) {
+        const int row = xrow0 + j * 8;
+        hx[j] = make_uint4(0, 0, 0, 0);
+        if (row < at.rows) fetch(hx[j], x + row * a.ldx, k0 + (lplace ^ C::xkey(row)) * 8);
+      }
+#pragma unroll
+      for (int j = 0; j < C::WI; ++j) {
+        const int row = wrow0 + j * 8;
+        hw[j] = make_uint4(0, 0, 0, 0);
+        if (row < cols) fetch(hw[j], w + row * a.ldw, k0 + (lplace ^ C::wkey(row)) * 8);
+      }
+    }
+  };
+  auto put = [&](int stage) {  // hx and hw into their places
+    if constexpr (!C::DMA) {
+#pragma unroll
+      for (int j = 0; j < C::XI; ++j) *(uint4*)(smem + dx + stage * C::STAGE + j * 1024 + lane * 16) = hx[j];
+#pragma unroll
+      for (int j = 0; j < C::WI; ++j) *(uint4*)(smem + dw + stage * C::STAGE + j * 1024 + lane * 16) = hw[j];
+    }
+  };
+
+  f32x4 acc[C::FI][C::FJ];
+#pragma unroll
+  for (int i = 0; i < C::FI; ++i)
+#pragma unroll
+    for (int j = 0; j < C::FJ; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  // fragment i's row r is column 32 (i / 2) + 8 (r / 4) + 4 (i % 2) + r % 4 of the wave: lane group q then holds
+  // columns 32 p + 8 q .. + 7 in fragments 2p and 2p + 1, and stores 16 bytes
+  const int fr = lane & 15, fq = lane >> 4;
+  const int xrow = wm + fr, wrow = wn + (fr >> 2) * 8 + (fr & 3);
+  const int ax[2] = {xrow * 128 + ((fq ^ C::xkey(xrow)) << 4), xrow * 128 + (((4 + fq) ^ C::xkey(xrow)) << 4)};
+  const int aw[2] = {(C::BM + wrow) * 128 + ((fq ^ C::wkey(wrow)) << 4),
+                     (C::BM + wrow) * 128 + (((4 + fq) ^ C::wkey(wrow)) << 4)};
+  auto read_x = [&](vec& v, int stage, int half, int j) {
+    v = *(const vec*)(smem + stage * C::STAGE + ax[half] + j * 16 * 128);
+  };
+  auto read_w = [&](vec& v, int stage, int half, int i) {
+    v = *(const vec*)(smem + stage * C::STAGE + aw[half] + ((i & 1) * 4 + (i >> 1) * 32) * 128);
+  };
+  vec fx[C::FJ], fa[C::FI], fb[C::FI];
+  // the products of one half, reading the next half's row fragments behind them
+  auto run = [&](vec(&f)[C::FI], bool more, int stage, int half) {
+#pragma unroll
+    for (int j = 0; j < C::FJ; ++j) {
+#pragma unroll
+      for (int i = 0; i < C::FI; ++i) acc[i][j] = Mfma<T>::run(f[i], fx[j], acc[i][j]);
+      if (more) read_x(fx[j], stage, half, j);
+    }
+  };
+  auto first = [&](int stage) {  // the first half of a slice
+#pragma unroll
+    for (int i = 0; i < C::FI; ++i) read_w(fb[i], stage, 1, i);
+    run(fa, true, stage, 1);
+  };
+
+  if (nk > 0) {
+    issue(0, 0);
+    put(0);
+    issue(1, 1);
+    put(1);
+    if constexpr (C::DMA) wait_vmcnt<C::XI + C::WI>();
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+#pragma unroll
+    for (int i = 0; i < C::FI; ++i) read_w(fa[i], 0, 0, i);
+#pragma unroll
+    for (int j = 0; j < C::FJ; ++j) read_x(fx[j], 0, 0, j);
+    for (int kt = 0; kt < nk - 1; ++kt) {
+      const int stage = kt & 1;
+      if constexpr (!C::DMA) issue(kt + 2, stage);
+      first(stage);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave is done reading `stage`
+      if constexpr (C::DMA) wait_vmcnt<0>();              // and slice kt + 1 is there
+      __builtin_amdgcn_s_barrier();
+#pragma unroll
+      for (int i = 0; i < C::FI; ++i) read_w(fa[i], stage ^ 1, 0, i);
+      if constexpr (C::DMA) issue(kt + 2, stage);
+      else put(stage);
+      run(fb, true, stage ^ 1, 0);
+    }
+    first((nk - 1) & 1);
+    run(fb, false, 0, 0);
+    if constexpr (C::DMA) wait_vmcnt<0>();  // slices past the last are zeros that still have to land
+  }
+  finish<C>(a, at, acc, wm, n0 + wn, lane);
+#endif
 }
 
 // row tiles that a grid needs: every group may end in a tile of its own
@@ -155,17 +381,28 @@ static long row_tiles(const DmlProductArgs* a, int bm) {
   return (a->M + (used + a->fill) * (bm - 1)) / bm;
 }
 
-template <class T>
+template <class C>
 static int launch(const DmlProductArgs* a, hipStream_t s) {
-  const long blocks = row_tiles(a, 64) * ((a->N + 63) / 64);
+  const long blocks = row_tiles(a, C::BM) * ((a->N + C::BN - 1) / C::BN);
   if (blocks > INT_MAX) {
     dml_set_error("dml_product: over 2^31 tiles");
     return -1;
   }
-  if (blocks == 0) return 0;
-  hipLaunchKernelGGL(product_simple<T>, dim3((unsigned)blocks), dim3(256), 0, s, *a);
+  hipLaunchKernelGGL(product_tile<C>, dim3((unsigned)blocks), dim3(C::NT), 0, s, *a);
   DML_CHECK_LAUNCH();
   return 0;
+}
+
+template <class T>
+static int dispatch(const DmlProductArgs* a, hipStream_t s) {
+  // LDS-DMA moves aligned 16 bytes at 32-bit offsets from a tile's first row
+  const bool dma = a->K % 8 == 0 && a->ldx % 8 == 0 && a->ldw % 8 == 0 && a->w_group % 8 == 0 &&
+                   (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) && a->K < (1 << 28);
+  const long big = row_tiles(a, 256) * ((a->N + 255) / 256), mid = row_tiles(a, 128) * ((a->N + 127) / 128);
+  if (!dma) return mid >= 256 ? launch<Tile<T, 128, 128, 2, 2, false>>(a, s) : launch<Tile<T, 64, 64, 2, 2, false>>(a, s);
+  if (big >= 512) return launch<Tile<T, 256, 256, 2, 4, true>>(a, s);
+  if (mid >= 256) return launch<Tile<T, 128, 128, 2, 2, true>>(a, s);
+  return launch<Tile<T, 64, 64, 2, 2, true>>(a, s);
 }
 
 }  // namespace prod
@@ -186,5 +423,5 @@ extern "C" int dml_product(const DmlProductArgs* a, hipStream_t s) {
     dml_set_error("dml_product: null tensor or row stride out of range");
     return -1;
   }
-  return a->dtype == DML_BF16 ? dml::prod::launch<bf16>(a, s) : dml::prod::launch<dml::f16>(a, s);
+  return a->dtype == DML_BF16 ? dml::prod::dispatch<bf16>(a, s) : dml::prod::dispatch<dml::f16>(a, s);
 }
