@@ -82,87 +82,129 @@ template <> struct Mfma<f16> {
   }
 };
 
-// Eight columns from `col` of one row through the epilogue; `n` of them exist.
-template <int KIND, class T>
-__device__ __forceinline__ void finish8(const DmlProductArgs& a, Act act, int64_t row, int col, int n, float (&v)[8],
-                                        const float (&bias)[8]) {
-  float r[8] = {};
-  if (a.res) {
-    if (a.out_f32) {
-      const float* p = (const float*)a.res + row * a.ldr + col;
-      if (n >= 8) __builtin_memcpy(r, p, 32);
-      else
-        for (int j = 0; j < 8; ++j)
-          if (j < n) r[j] = p[j];
-    } else {
-      const T* p = (const T*)a.res + row * a.ldr + col;
-      T t[8] = {};
-      if (n >= 8) __builtin_memcpy(t, p, 16);
-      else
-        for (int j = 0; j < 8; ++j)
-          if (j < n) t[j] = p[j];
+// One output element: column `col` of row `row`, in group e.
+template <class T>
+__device__ __forceinline__ void finish1(const DmlProductArgs& a, int e, int64_t row, int col, float v) {
+  if (a.bias) v += a.bias[e * a.bias_group + col];
+  float r = 0.f;
+  if (a.res)
+    r = a.out_f32 ? ((const float*)a.res)[row * a.ldr + col] : to_f32(((const T*)a.res)[row * a.ldr + col]);
+  v = a.act_last ? activate(v + r, a.act) : activate(v, a.act) + r;
+  if (a.out_f32) ((float*)a.y)[row * a.ldy + col] = v;
+  else ((T*)a.y)[row * a.ldy + col] = (T)v;
+}
+
+// Bias of the eight columns that a lane holds in each pair of its wave's column fragments.
+template <class C>
+struct Bias {
+  float v[C::FI / 2][8];
+  __device__ __forceinline__ void load(const DmlProductArgs& a, int e, int col0, int lane) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) r[j] = to_f32(t[j]);
+    for (int p = 0; p < C::FI / 2; ++p) {
+      const int col = col0 + p * 32 + (lane >> 4) * 8;
+      const float* b = a.bias + e * a.bias_group;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[p][j] = a.bias && col + j < a.N ? b[col + j] : 0.f;
     }
   }
+};
+
+// A wave's accumulators (rows wm.., columns col0.., all of them inside) through the epilogue: of its 16 x 32 pieces
+// those whose number is `mine` modulo `of`. A lane has eight columns of a row in a piece. The residuals of four pieces
+// are read ahead of the stores, which could be to the same memory.
+template <int KIND, class C>
+__device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ],
+                                          const Bias<C>& bias, int wm, int col0, int lane, int mine, int of) {
+  typedef typename C::T T;
+  const Act act = act_parameters(a.act);
+  constexpr int G = C::FJ < 4 ? C::FJ : 4;
+  const int m0 = wm + (lane & 15);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] += bias[j];
-  if (a.act_last) {
+  for (int p = 0; p < C::FI / 2; ++p) {
+    const int64_t col = col0 + p * 32 + (lane >> 4) * 8;
+    const int64_t y0 = (at.row + m0) * a.ldy + col, r0 = (at.row + m0) * a.ldr + col;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = act.run<KIND>(v[j] + r[j]);
-  } else {
+    for (int j0 = 0; j0 < C::FJ; j0 += G) {
+      float r[G][8] = {};
+      if (a.res) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = act.run<KIND>(v[j]) + r[j];
-  }
-  if (a.out_f32) {
-    float* p = (float*)a.y + row * a.ldy + col;
-    if (n >= 8) __builtin_memcpy(p, v, 32);
-    else
-      for (int j = 0; j < 8; ++j)
-        if (j < n) p[j] = v[j];
-  } else {
-    T* p = (T*)a.y + row * a.ldy + col;
-    T t[8];
+        for (int j = 0; j < G; ++j)
+          if (m0 + (j0 + j) * 16 < at.rows) {
+            const int64_t i = r0 + (j0 + j) * 16 * a.ldr;
+            if (a.out_f32) {
+              __builtin_memcpy(r[j], (const float*)a.res + i, 32);
+            } else {
+              Vec16<T> t;
+              t.load((const T*)a.res + i);
+              t.get(r[j]);
+            }
+          }
+      }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = (T)v[j];
-    if (n >= 8) __builtin_memcpy(p, t, 16);
-    else
-      for (int j = 0; j < 8; ++j)
-        if (j < n) p[j] = t[j];
+      for (int j = 0; j < G; ++j) {
+        if ((p * C::FJ + j0 + j) % of != mine || m0 + (j0 + j) * 16 >= at.rows) continue;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = acc[2 * p + q / 4][j0 + j][q % 4] + bias.v[p][q];
+        if (a.act_last) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = act.run<KIND>(v[q] + r[j][q]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = act.run<KIND>(v[q]) + r[j][q];
+        }
+        const int64_t i = y0 + (j0 + j) * 16 * a.ldy;
+        if (a.out_f32) {
+          __builtin_memcpy((float*)a.y + i, v, 32);
+        } else {
+          Vec16<T> t;
+          t.set(v);
+          t.store((T*)a.y + i);
+        }
+      }
+    }
   }
 }
 
-// A wave's accumulators (rows wm.., columns col0..) through the epilogue.
-template <int KIND, class C>
-__device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
-                                          int col0, int lane) {
-  const Act act = act_parameters(a.act);
+// The same where columns of the tile lie past N: 16 rows at a time through `lds` (64 bytes a column), element by
+// element in the columns' order.
+template <class C>
+__device__ __forceinline__ void finish_ragged(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
+                                              int col0, int lane, int mine, int of, float* lds) {
 #pragma unroll
-  for (int p = 0; p < C::FI / 2; ++p) {
-    const int col = col0 + p * 32 + (lane >> 4) * 8, n = a.N - col;
-    float bias[8];
+  for (int j = 0; j < C::FJ; ++j) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) bias[j] = a.bias && j < n ? a.bias[at.e * a.bias_group + col + j] : 0.f;
+    for (int p = 0; p < C::FI / 2; ++p) {
+      if ((p * C::FJ + j) % of != mine) continue;
+      const int c = p * 32 + (lane >> 4) * 8;
 #pragma unroll
-    for (int j = 0; j < C::FJ; ++j) {
-      const int m = wm + j * 16 + (lane & 15);
-      float v[8];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        v[q] = acc[2 * p][j][q];
-        v[4 + q] = acc[2 * p + 1][j][q];
+      for (int q = 0; q < 8; ++q) lds[(lane & 15) * C::TN + c + q] = acc[2 * p + q / 4][j][q % 4];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int i = lane; i < 16 * 32; i += 64) {
+        const int m = wm + j * 16 + i / 32, col = col0 + p * 32 + i % 32;
+        if (m < at.rows && col < a.N)
+          finish1<typename C::T>(a, at.e, (int64_t)at.row + m, col, lds[i / 32 * C::TN + p * 32 + i % 32]);
       }
-      if (m < at.rows && n > 0) finish8<KIND, typename C::T>(a, act, (int64_t)at.row + m, col, n, v, bias);
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
 
 template <class C>
-__device__ __forceinline__ void finish(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
-                                       int col0, int lane) {
-  if (a.act <= DML_ACT_RELU) finish_as<kClamp, C>(a, at, acc, wm, col0, lane);
-  else if (a.act == DML_ACT_GELU) finish_as<kErf, C>(a, at, acc, wm, col0, lane);
-  else finish_as<kSwish, C>(a, at, acc, wm, col0, lane);
+__device__ __forceinline__ void finish(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ],
+                                       const Bias<C>& bias, int wm, int n0, int wn, int lane, int mine, int of, char* lds,
+                                       int wave) {
+  if (n0 + C::BN > a.N) {
+    __syncthreads();
+    finish_ragged<C>(a, at, acc, wm, n0 + wn, lane, mine, of, (float*)lds + wave * 16 * C::TN);
+  } else if (a.act <= DML_ACT_RELU) {
+    finish_as<kClamp, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+  } else if (a.act == DML_ACT_GELU) {
+    finish_as<kErf, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+  } else {
+    finish_as<kSwish, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+  }
 }
 
 // Zeros into rows wm .. wm + rows, columns col0 .. col0 + cols of a tile.
@@ -188,17 +230,22 @@ __device__ __forceinline__ void zero_rows(const DmlProductArgs& a, const Place& 
 //
 // 16-byte chunks lie in a tile row XORed with a key of the row, chosen so that the lanes that LDS serves together
 // (0-3, 12-15, 20-23, 24-27 and so on) hit all 64 banks with both operands' row patterns: no conflicts by the counters.
-template <class T_, int BM_, int BN_, int WM_, int WN_, bool DMA_>
+//
+// KG > 1: KG such sets of waves, each with LDS of its own, take the slices in turn; their sums meet in LDS at the end
+// and are added in the sets' order. Where there are few tiles this is what fills the CUs (256 x 4096 x 4096: 32 us
+// with one set, 20 with four).
+template <class T_, int BM_, int BN_, int WM_, int WN_, int KG_, bool DMA_>
 struct Tile {
   typedef T_ T;
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, BK = 64;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KG = KG_, BK = 64;
   static constexpr bool DMA = DMA_;
-  static constexpr int NW = WM * WN, NT = NW * 64;
+  static constexpr int NW = WM * WN, NT = KG * NW * 64;       // waves of a set, threads
   static constexpr int TM = BM / WM, TN = BN / WN;            // rows, columns of a wave
   static constexpr int FJ = TM / 16, FI = TN / 16;            // fragments along rows, columns
   static constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW;    // pieces of 8 tile rows that a wave copies per slice
-  static constexpr int STAGE = (BM + BN) * 128, LDS = 2 * STAGE;
-  static constexpr int MINW = (LDS <= 40960 ? 4 : LDS <= 81920 ? 2 : 1) * NW / 4;  // waves a SIMD that LDS leaves room for
+  static constexpr int STAGE = (BM + BN) * 128, LDS = KG * 2 * STAGE;
+  static constexpr int MINW = (LDS <= 40960 ? 4 : LDS <= 81920 ? 2 : 1) * KG * NW / 4;  // waves a SIMD that LDS leaves room for
+  static_assert(KG == 1 || BM * BN * 4 <= 2 * STAGE, "a set's sums fit its LDS");
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && TN % 32 == 0 && TM % 16 == 0 && LDS <= 163840, "tile");
   __device__ __forceinline__ static int xkey(int row) { return row & 7; }
   __device__ __forceinline__ static int wkey(int row) { return (row & 3) | ((row >> 1) & 4); }
@@ -211,7 +258,7 @@ __global__ __launch_bounds__(C::NT, C::MINW) void product_tile(DmlProductArgs a)
 #ifdef __HIP_DEVICE_COMPILE__  // the host needs the entry only
   typedef typename C::T T;
   typedef typename Mfma<T>::vec vec;
-  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];
+  __shared__ __attribute__((aligned(1024))) char all[C::LDS];
   // blocks of one XCD take neighbouring tiles, eight row tiles by all column tiles at a time
   const int ntn = (a.N + C::BN - 1) / C::BN, nb = gridDim.x;
   const int b = xcd_remap(blockIdx.x, nb), s0 = b / (8 * ntn) * 8;
@@ -220,13 +267,15 @@ __global__ __launch_bounds__(C::NT, C::MINW) void product_tile(DmlProductArgs a)
   const Place at = locate<C::BM>(a, tm);
   if (at.rows <= 0) return;
   const int n0 = tn * C::BN, cols = a.N - n0;
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave / C::NW, wid = wave % C::NW;
   const int wm = wid / C::WN * C::TM, wn = wid % C::WN * C::TN;
   if (at.e >= a.E) {
-    zero_rows<T>(a, at, n0 + wn, C::TN, wm, C::TM, lane);
+    if (kg == 0) zero_rows<T>(a, at, n0 + wn, C::TN, wm, C::TM, lane);
     return;
   }
-  const int nk = (a.K + C::BK - 1) / C::BK;
+  const int nk = (a.K + C::KG * C::BK - 1) / (C::KG * C::BK);  // slices of a set; those past K are zeros
+  char* const smem = all + kg * 2 * C::STAGE;
   const T* const x = (const T*)a.x + at.row * a.ldx;
   const T* const w = (const T*)a.w + at.e * a.w_group + (int64_t)n0 * a.ldw;
 
@@ -264,7 +313,7 @@ __global__ __launch_bounds__(C::NT, C::MINW) void product_tile(DmlProductArgs a)
   };
   // request slice kt: by DMA into `stage`, or into hx and hw
   auto issue = [&](int kt, int stage) {
-    const int k0 = kt * C::BK;
+    const int k0 = (kt * C::KG + kg) * C::BK;
     if constexpr (C::DMA) {
       if (k0 + C::BK > a.K) {  // chunks past K are out from now on
 #pragma unroll
@@ -326,6 +375,7 @@ __global__ __launch_bounds__(C::NT, C::MINW) void product_tile(DmlProductArgs a)
     v = *(const vec*)(smem + stage * C::STAGE + aw[half] + ((i & 1) * 4 + (i >> 1) * 32) * 128);
   };
   vec fx[C::FJ], fa[C::FI], fb[C::FI];
+  Bias<C> bias;
   // the products of one half, reading the next half's row fragments behind them
   auto run = [&](vec(&f)[C::FI], bool more, int stage, int half) {
 #pragma unroll
@@ -366,11 +416,111 @@ __global__ __launch_bounds__(C::NT, C::MINW) void product_tile(DmlProductArgs a)
       else put(stage);
       run(fb, true, stage ^ 1, 0);
     }
+    bias.load(a, at.e, n0 + wn, lane);  // in flight over the last slice
     first((nk - 1) & 1);
     run(fb, false, 0, 0);
     if constexpr (C::DMA) wait_vmcnt<0>();  // slices past the last are zeros that still have to land
+  } else {
+    bias.load(a, at.e, n0 + wn, lane);
   }
-  finish<C>(a, at, acc, wm, n0 + wn, lane);
+  if constexpr (C::KG == 1) {
+    finish<C>(a, at, acc, bias, wm, n0, wn, lane, 0, 1, all, wave);
+  } else {
+    __syncthreads();
+    f32x4* const sums = (f32x4*)all;  // [set][wave][fragment][lane]
+    constexpr int F = C::FI * C::FJ;
+#pragma unroll
+    for (int i = 0; i < C::FI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FJ; ++j) sums[((kg * C::NW + wid) * F + i * C::FJ + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < C::FI; ++i)
+#pragma unroll
+      for (int j = 0; j < C::FJ; ++j)
+        if (((i / 2) * C::FJ + j) % C::KG == kg) {
+          acc[i][j] = sums[(wid * F + i * C::FJ + j) * 64 + lane];
+#pragma unroll
+          for (int g = 1; g < C::KG; ++g) acc[i][j] += sums[((g * C::NW + wid) * F + i * C::FJ + j) * 64 + lane];
+        }
+    finish<C>(a, at, acc, bias, wm, n0, wn, lane, kg, C::KG, all, wave);
+  }
+#endif
+}
+
+// ---- few rows: K split over the waves ----
+//
+// A workgroup of NW waves computes 16 MF rows x 16 NF columns; the waves take the K slices of 64 in turn and load their
+// fragments straight from memory (any alignment): with few rows the weight is read once, in order, and nothing is
+// shared but the end, where the waves' sums meet in LDS and are added in the waves' order. Bound by the weight's bytes
+// (one row, 2048 x 1000) or by the latency of a few loads in a row, so a wave keeps U slices in flight.
+template <class T, int MF, int NF, int NW, int U>
+__global__ __launch_bounds__(NW * 64) void product_rows(DmlProductArgs a) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host needs the entry only
+  typedef typename Mfma<T>::vec vec;
+  constexpr int F = MF * NF;
+  __shared__ f32x4 part[NW][F][64];
+  const int ntn = (a.N + NF * 16 - 1) / (NF * 16);
+  const int b = xcd_remap(blockIdx.x, gridDim.x), tm = b / ntn, n0 = (b - tm * ntn) * NF * 16;
+  const Place at = locate<MF * 16>(a, tm);
+  if (at.rows <= 0) return;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at.e >= a.E) {
+    if (wid == 0) zero_rows<T>(a, at, n0, NF * 16, 0, MF * 16, lane);
+    return;
+  }
+  const int fr = lane & 15, fq = lane >> 4;
+  const T* const x = (const T*)a.x + (at.row + fr) * a.ldx;
+  const T* const w = (const T*)a.w + at.e * a.w_group + (n0 + fr) * a.ldw;
+  auto fetch = [&](vec& v, const T* p, int k, bool row) {  // eight values from k of a row; 0 outside
+    if (row && k + 8 <= a.K) {
+      __builtin_memcpy(&v, p + k, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = row && k + i < a.K ? p[k + i] : (T)0.f;
+    }
+  };
+  f32x4 acc[MF][NF];
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int n = 0; n < NF; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wid * 64; k0 < a.K; k0 += NW * 64 * U) {
+    vec fx[U][2][MF], fw[U][2][NF];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + u * NW * 64 + h * 32 + fq * 8;
+#pragma unroll
+        for (int n = 0; n < NF; ++n) fetch(fw[u][h][n], w + n * 16 * a.ldw, k, n0 + n * 16 + fr < a.N);
+#pragma unroll
+        for (int m = 0; m < MF; ++m) fetch(fx[u][h][m], x + m * 16 * a.ldx, k, m * 16 + fr < at.rows);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < MF; ++m)
+#pragma unroll
+          for (int n = 0; n < NF; ++n) acc[m][n] = Mfma<T>::run(fw[u][h][n], fx[u][h][m], acc[m][n]);
+  }
+#pragma unroll
+  for (int m = 0; m < MF; ++m)
+#pragma unroll
+    for (int n = 0; n < NF; ++n) part[wid][m * NF + n][lane] = acc[m][n];
+  __syncthreads();
+  for (int f = wid; f < F; f += NW) {
+    f32x4 v = part[0][f][lane];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) v += part[i][f][lane];
+    const int m = f / NF * 16 + fr, col = n0 + f % NF * 16 + fq * 4;
+    if (m >= at.rows) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (col + q < a.N) finish1<T>(a, at.e, (int64_t)at.row + m, col + q, v[q]);
+  }
 #endif
 }
 
@@ -394,15 +544,60 @@ static int launch(const DmlProductArgs* a, hipStream_t s) {
 }
 
 template <class T>
+static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
+  const long blocks = row_tiles(a, 16) * ((a->N + 15) / 16);
+  if (blocks > INT_MAX) {
+    dml_set_error("dml_product: over 2^31 tiles");
+    return -1;
+  }
+  hipLaunchKernelGGL((product_rows<T, 1, 1, 16, 2>), dim3((unsigned)blocks), dim3(1024), 0, s, *a);
+  DML_CHECK_LAUNCH();
+  return 0;
+}
+
+// The forms a product can run in, and what each costs in microseconds: `fixed` a tile (the epilogue), and a slice of 64
+// (KG of them) `alone` where a CU has one such workgroup at a time, `shared` times their number where it has more (the
+// L2's rate, or the matrix cores' for the largest). Measured over 1 to 16384 rows, K 256 to 8192, N 256 to 8192
+// (256 x 4096 x 4096: 32.2 / 24.1 / 20.1 us with KG 1 / 2 / 4; 1024 x 512 x 2048: 7.6 / 8.6 / 11.3; 16384 x 1024 x
+// 4096: 156 us in tiles of 256, 166 of 128; 6304 x 4096 x 1024: 94 and 57).
+struct Form {
+  int bm, bn, kg, per_cu;
+  double fixed, alone, shared;
+};
+constexpr Form kForms[] = {{64, 64, 1, 4, 1.0, 0.47, 0.25}, {64, 64, 2, 2, 1.5, 0.68, 0.5}, {64, 64, 4, 1, 2.5, 1.1, 1.1},
+                           {128, 128, 1, 2, 3.0, 0.65, 0.46}, {256, 256, 1, 1, 11.0, 1.6, 1.6}};
+
+static double cost(const DmlProductArgs* a, const Form& f) {
+  const double tiles = (double)row_tiles(a, f.bm) * ((a->N + f.bn - 1) / f.bn);
+  const long per = (long)((tiles + 255) / 256), rounds = per / f.per_cu, rest = per % f.per_cu;
+  const auto slice = [&](long n) { return n == 0 ? 0.0 : n * f.shared > f.alone ? n * f.shared : f.alone; };
+  const int slices = (a->K + 64 * f.kg - 1) / (64 * f.kg);
+  return slices * (rounds * slice(f.per_cu) + slice(rest)) + per * f.fixed;
+}
+
+template <class T>
 static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   // LDS-DMA moves aligned 16 bytes at 32-bit offsets from a tile's first row
   const bool dma = a->K % 8 == 0 && a->ldx % 8 == 0 && a->ldw % 8 == 0 && a->w_group % 8 == 0 &&
-                   (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) && a->K < (1 << 28);
-  const long big = row_tiles(a, 256) * ((a->N + 255) / 256), mid = row_tiles(a, 128) * ((a->N + 127) / 128);
-  if (!dma) return mid >= 256 ? launch<Tile<T, 128, 128, 2, 2, false>>(a, s) : launch<Tile<T, 64, 64, 2, 2, false>>(a, s);
-  if (big >= 512) return launch<Tile<T, 256, 256, 2, 4, true>>(a, s);
-  if (mid >= 256) return launch<Tile<T, 128, 128, 2, 2, true>>(a, s);
-  return launch<Tile<T, 64, 64, 2, 2, true>>(a, s);
+                   (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) &&
+                   a->K < (1 << 28);
+  // product_rows: a column tile's weight in one pass, 3.5 us per 2048 of K and workgroup on a CU
+  const double tiles = (double)row_tiles(a, 16) * ((a->N + 15) / 16), k = a->K / 2048.0;
+  double least = (double)(long)((tiles + 255) / 256) * (k < 0.45 ? 0.45 : k) * 3.5 + 0.5;
+  int best = -1;
+  for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
+    if (!dma && (kForms[i].bm == 256 || kForms[i].kg == 2)) continue;  // not built through registers
+    const double c = cost(a, kForms[i]);
+    if (c < least) least = c, best = i;
+  }
+  switch (best) {
+    case -1: return launch_rows<T>(a, s);
+    case 0: return dma ? launch<Tile<T, 64, 64, 2, 2, 1, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 1, false>>(a, s);
+    case 1: return launch<Tile<T, 64, 64, 2, 2, 2, true>>(a, s);
+    case 2: return dma ? launch<Tile<T, 64, 64, 2, 2, 4, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 4, false>>(a, s);
+    case 3: return dma ? launch<Tile<T, 128, 128, 2, 2, 1, true>>(a, s) : launch<Tile<T, 128, 128, 2, 2, 1, false>>(a, s);
+    default: return launch<Tile<T, 256, 256, 2, 4, 1, true>>(a, s);
+  }
 }
 
 }  // namespace prod
