@@ -121,8 +121,8 @@ class ProductArgs(C.Structure):
 
 
 _SIGS = {
-    "dml_group_norm": (C.c_int64, [C.POINTER(GroupNormArgs), C.c_void_p]),
-    "dml_product": (C.c_int, [C.POINTER(ProductArgs), C.c_void_p]),
+    "dml_group_norm": (C.c_int64, [C.c_void_p, C.c_void_p]),
+    "dml_product": (C.c_int, [C.c_void_p, C.c_void_p]),
     "dml_expand_reduce": (C.c_int, [C.POINTER(ExpandReduceArgs), C.c_void_p]),
     "dml_chain_supported": (C.c_int, [C.POINTER(ExpandReduceArgs)]),
     "dml_plan_add_expand_reduce": (C.c_int, [C.c_void_p, C.POINTER(ExpandReduceArgs)]),

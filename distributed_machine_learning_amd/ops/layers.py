@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -18,20 +19,27 @@ from .. import _native as N
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # DML_ACT_*
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # DML_BF16, DML_F16, DML_F32
 _INT = 2 ** 31 - 1
+# N.GroupNormArgs and N.ProductArgs as packed bytes: a call of small tensors is bound by the host, and filling the
+# ctypes structures took a microsecond more
+_NORM, _PROD = struct.Struct("@4P4qPq6if4x"), struct.Struct("@6P6q10i")
+assert (_NORM.size, _PROD.size) == (C.sizeof(N.GroupNormArgs), C.sizeof(N.ProductArgs))
 
 
 def _act(act: str) -> int:
-    try:
-        return ACTIVATIONS[act]
-    except (KeyError, TypeError):
-        raise ValueError(f"act is one of {', '.join(ACTIVATIONS)}: got {act!r}") from None
+    code = ACTIVATIONS.get(act)
+    if code is None:
+        raise ValueError(f"act is one of {', '.join(ACTIVATIONS)}: got {act!r}")
+    return code
 
 
 def _pitch(t: torch.Tensor, first: int, what: str) -> Tuple[int, int]:
     """(rows, elements from one row to the next) of dimensions first .. -2 of t seen as rows of its last one."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
     if t.is_contiguous():
+        if len(shape) == first + 2:
+            return shape[first], shape[first + 1]
         return math.prod(shape[first:-1]), shape[-1]
+    stride = t.stride()
     if shape[-1] > 1 and stride[-1] != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous, got strides {stride}")
     rows, pitch = 1, None
@@ -73,37 +81,37 @@ def _apart(out: torch.Tensor, t: Optional[torch.Tensor], what: str, same: bool =
     raise ValueError(f"out overlaps {what}")
 
 
-def _vector(v: Optional[torch.Tensor], shape: Tuple[int, ...], dtype: torch.dtype, what: str) -> None:
-    if v is None:
-        return
-    if tuple(v.shape) != shape:
+def _vector(v: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, what: str) -> None:
+    if v.shape != shape:
         raise ValueError(f"{what}: expected shape {shape}, got {tuple(v.shape)}")
     if v.dtype is not torch.float32 and v.dtype is not dtype:
         raise TypeError(f"{what}: expected float32 or {dtype}, got {v.dtype}")
 
 
-def _ready(*tensors: Optional[torch.Tensor]) -> None:
-    """All on one HIP device, and none that autograd would expect a gradient for."""
-    dev = tensors[0].device
+def _ready(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """x's device number: all are on one HIP device, and none is one that autograd would expect a gradient for."""
+    dev = x.get_device()
     grad = torch.is_grad_enabled()
-    for t in tensors:
+    if grad and x.requires_grad:
+        raise ValueError("this operator has no backward: call it under torch.no_grad()")
+    for t in others:
         if t is not None:
-            if t.device != dev:
-                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+            if t.get_device() != dev or (dev < 0 and t.device != x.device):
+                raise ValueError(f"tensors on different devices: {x.device} and {t.device}")
             if grad and t.requires_grad:
                 raise ValueError("this operator has no backward: call it under torch.no_grad()")
-    if dev.type != "cuda":
-        raise ValueError(f"expected tensors on a HIP device, got {dev}")
+    if dev < 0:
+        raise ValueError(f"expected tensors on a HIP device, got {x.device}")
+    return dev
 
 
-def _launch(fn, a, device: torch.device, what: str) -> int:
-    """fn(a, the current stream of device), with device current."""
-    i = device.index
-    if i == torch.cuda.current_device():
-        rc = fn(C.byref(a), torch._C._cuda_getCurrentRawStream(i))
+def _launch(fn, args: bytes, device: int, what: str) -> int:
+    """fn(args, the current stream of device), with device current."""
+    if device == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(i):
-            rc = fn(C.byref(a), torch._C._cuda_getCurrentRawStream(i))
+        with torch.cuda.device(device):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(device))
     return N.check(rc, what) if rc else 0
 
 
@@ -123,17 +131,21 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     act: "none", "relu", "silu", "gelu" or "gelu_tanh". out: x's shape and type; may be x itself.
     """
     code = _act(act)
-    if x.dtype not in _DTYPES:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
         raise TypeError(f"x: expected bfloat16, float16 or float32, got {x.dtype}")
-    if x.dim() < 2:
-        raise ValueError(f"x: expected [N, ..., C], got shape {tuple(x.shape)}")
-    n, c = x.shape[0], x.shape[-1]
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"x: expected [N, ..., C], got shape {tuple(shape)}")
+    n, c = shape[0], shape[-1]
     if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or c < 1 or c % groups:
         raise ValueError(f"groups must divide the {c} channels, got {groups!r}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    _vector(weight, (c,), x.dtype, "weight")
-    _vector(bias, (c,), x.dtype, "bias")
+    if weight is not None:
+        _vector(weight, (c,), x.dtype, "weight")
+    if bias is not None:
+        _vector(bias, (c,), x.dtype, "bias")
     rows, ldx = _pitch(x, 1, "x")
     if out is None:
         ldy = c
@@ -148,53 +160,55 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         _apart(out, bias, "bias")
     if n > _INT or rows > _INT or n * groups > _INT:
         raise ValueError("x: over 2^31 - 1 samples, positions or groups")
-    _ready(x, weight, bias, out)
+    device = _ready(x, weight, bias, out)
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    if not out.numel():
+        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+    if not (n and rows):
         return out
     weight, bias = _f32(weight), _f32(bias)
-    a = N.GroupNormArgs(x.data_ptr(), out.data_ptr(), weight.data_ptr() if weight is not None else None,
-                        bias.data_ptr() if bias is not None else None, x.stride(0), out.stride(0),
-                        ldx, ldy, None, 0, n, rows, c, groups, _DTYPES[x.dtype], code, eps)
-    fn = N.lib().dml_group_norm
-    need = _launch(fn, a, x.device, "dml_group_norm")
-    if need:
+    ws, need, fn = None, 0, N.lib().dml_group_norm
+    while True:
+        need = _launch(fn, _NORM.pack(
+            x.data_ptr(), out.data_ptr(), 0 if weight is None else weight.data_ptr(),
+            0 if bias is None else bias.data_ptr(), x.stride(0), out.stride(0), ldx, ldy,
+            0 if ws is None else ws.data_ptr(), need, n, rows, c, groups, dtype, code, eps), device, "dml_group_norm")
+        if not need:
+            return out
         ws = torch.empty(need, device=x.device, dtype=torch.uint8)
-        a.ws, a.ws_bytes = ws.data_ptr(), need
-        _launch(fn, a, x.device, "dml_group_norm")
-    return out
 
 
 def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, what):
     code = _act(act)
-    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
-        raise TypeError(f"x: expected bfloat16 or float16, got {x.dtype}")
-    if weight.dtype is not x.dtype:
-        raise TypeError(f"weight: expected {x.dtype} like x, got {weight.dtype}")
+    dtype = x.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError(f"x: expected bfloat16 or float16, got {dtype}")
+    if weight.dtype is not dtype:
+        raise TypeError(f"weight: expected {dtype} like x, got {weight.dtype}")
+    xs, wsh = x.shape, weight.shape
     wdim = 2 if ends is None else 3
-    if weight.dim() != wdim or x.dim() < 1 or weight.shape[-1] != x.shape[-1]:
-        raise ValueError(f"{what}: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
-    n, k = weight.shape[-2], weight.shape[-1]
-    e = 1 if ends is None else weight.shape[0]
-    shape = (*x.shape[:-1], n)
-    to = out.dtype if out is not None else out_dtype if out_dtype is not None else x.dtype
-    if to is not x.dtype and to is not torch.float32:
-        raise TypeError(f"out: expected {x.dtype} or float32, got {to}")
+    if len(wsh) != wdim or not xs or wsh[-1] != xs[-1]:
+        raise ValueError(f"{what}: x {tuple(xs)} does not fit weight {tuple(wsh)}")
+    n, k = wsh[-2:]
+    e = 1 if ends is None else wsh[0]
+    shape = (*xs[:-1], n)
+    to = out.dtype if out is not None else out_dtype if out_dtype is not None else dtype
+    if to is not dtype and to is not torch.float32:
+        raise TypeError(f"out: expected {dtype} or float32, got {to}")
     if out_dtype is not None and out_dtype is not to:
         raise TypeError(f"out is {to}, out_dtype {out_dtype}")
-    _vector(bias, (n,) if ends is None else (e, n), x.dtype, "bias")
+    if bias is not None:
+        _vector(bias, (n,) if ends is None else (e, n), dtype, "bias")
     m, ldx = _pitch(x, 0, "x")
     _, ldw = _pitch(weight, wdim - 2, "weight")
+    ldr = 0
     if residual is not None:
-        if tuple(residual.shape) != shape or residual.dtype is not to:
+        if residual.shape != shape or residual.dtype is not to:
             raise ValueError(f"residual: expected {to} of shape {shape}, got {residual.dtype} of "
                              f"{tuple(residual.shape)}")
         ldr = _pitch(residual, 0, "residual")[1]
-    if out is None:
-        ldy = n
-    else:
-        if tuple(out.shape) != shape:
+    ldy = n
+    if out is not None:
+        if out.shape != shape:
             raise ValueError(f"out: expected shape {shape}, got {tuple(out.shape)}")
         ldy = _pitch(out, 0, "out")[1]
         if m > 1 and ldy < n:
@@ -206,23 +220,21 @@ def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, wha
         _apart(out, residual, "residual", same=True)
     if max(m, n, k, e) > _INT - 512:
         raise ValueError(f"{what}: a dimension over 2^31 - 513")
-    _ready(x, weight, ends, bias, residual, out)
+    device = _ready(x, weight, ends, bias, residual, out)
     fill = 0
     if out is None:
         out = torch.empty(shape, device=x.device, dtype=to)
         fill = int(ends is not None)
-    if not out.numel():
+    if not (m and n):
         return out
     if e == 0:
         return out.zero_() if fill else out
     bias = _f32(bias)
-    a = N.ProductArgs(x.data_ptr(), weight.data_ptr(), bias.data_ptr() if bias is not None else None,
-                      residual.data_ptr() if residual is not None else None, out.data_ptr(),
-                      ends.data_ptr() if ends is not None else None, ldx, ldw,
-                      weight.stride(0) if wdim == 3 else 0, n, ldr if residual is not None else 0, ldy,
-                      m, n, k, e, _DTYPES[x.dtype], int(to is torch.float32), code, int(bool(act_last)),
-                      int(ends is not None and ends.dtype is torch.int64), fill)
-    _launch(N.lib().dml_product, a, x.device, what)
+    _launch(N.lib().dml_product, _PROD.pack(
+        x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if residual is None else residual.data_ptr(), out.data_ptr(), 0 if ends is None else ends.data_ptr(),
+        ldx, ldw, weight.stride(0) if wdim == 3 else 0, n, ldr, ldy, m, n, k, e, _DTYPES[dtype],
+        to is torch.float32, code, bool(act_last), ends is not None and ends.dtype is torch.int64, fill), device, what)
     return out
 
 
