@@ -472,12 +472,30 @@ __global__ __launch_bounds__(NW * 64) void product_rows(DmlProductArgs a) {
   const int fr = lane & 15, fq = lane >> 4;
   const T* const x = (const T*)a.x + (at.row + fr) * a.ldx;
   const T* const w = (const T*)a.w + at.e * a.w_group + (n0 + fr) * a.ldw;
-  auto fetch = [&](vec& v, const T* p, int k, bool row) {  // eight values from k of a row; 0 outside
+  // Rows that start in the middle of a dword (the lane's rows are 16 apart: all of them or none) are loaded from the
+  // dword's start and shifted: 16-byte loads off the dword grid took 1.7 times as long (1 x 4001 x 2000: 15 us, 9 for
+  // 4002). The value ahead of the row shares its dword with the first.
+  const bool oddx = ((uintptr_t)x & 2) != 0, oddw = ((uintptr_t)w & 2) != 0;
+  auto fetch = [&](vec& v, const T* p, int k, bool row, bool odd) {  // eight values from k of a row; 0 outside
     if (row && k + 8 <= a.K) {
-      __builtin_memcpy(&v, p + k, 16);
+      uint4 u;
+      __builtin_memcpy(&u, p + k - (odd ? 1 : 0), 16);
+      if (odd) {
+        const unsigned last = *(const unsigned short*)(p + k + 7);
+        u.x = __builtin_amdgcn_alignbyte(u.y, u.x, 2);
+        u.y = __builtin_amdgcn_alignbyte(u.z, u.y, 2);
+        u.z = __builtin_amdgcn_alignbyte(u.w, u.z, 2);
+        u.w = __builtin_amdgcn_alignbyte(last, u.w, 2);
+      }
+      __builtin_memcpy(&v, &u, 16);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = row && k + i < a.K ? p[k + i] : (T)0.f;
+      for (int i = 0; i < 8; ++i) v[i] = (T)0.f;
+      if (row && k < a.K) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < a.K) v[i] = p[k + i];
+      }
     }
   };
   f32x4 acc[MF][NF];
@@ -493,9 +511,9 @@ __global__ __launch_bounds__(NW * 64) void product_rows(DmlProductArgs a) {
       for (int h = 0; h < 2; ++h) {
         const int k = k0 + u * NW * 64 + h * 32 + fq * 8;
 #pragma unroll
-        for (int n = 0; n < NF; ++n) fetch(fw[u][h][n], w + n * 16 * a.ldw, k, n0 + n * 16 + fr < a.N);
+        for (int n = 0; n < NF; ++n) fetch(fw[u][h][n], w + n * 16 * a.ldw, k, n0 + n * 16 + fr < a.N, oddw);
 #pragma unroll
-        for (int m = 0; m < MF; ++m) fetch(fx[u][h][m], x + m * 16 * a.ldx, k, m * 16 + fr < at.rows);
+        for (int m = 0; m < MF; ++m) fetch(fx[u][h][m], x + m * 16 * a.ldx, k, m * 16 + fr < at.rows, oddx);
       }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -543,36 +561,38 @@ static int launch(const DmlProductArgs* a, hipStream_t s) {
   return 0;
 }
 
-template <class T>
+template <class T, int F, int NW, int U>
 static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
-  const long blocks = row_tiles(a, 16) * ((a->N + 15) / 16);
+  const long blocks = row_tiles(a, 16 * F) * ((a->N + 16 * F - 1) / (16 * F));
   if (blocks > INT_MAX) {
     dml_set_error("dml_product: over 2^31 tiles");
     return -1;
   }
-  hipLaunchKernelGGL((product_rows<T, 1, 1, 16, 2>), dim3((unsigned)blocks), dim3(1024), 0, s, *a);
+  hipLaunchKernelGGL((product_rows<T, F, F, NW, U>), dim3((unsigned)blocks), dim3(NW * 64), 0, s, *a);
   DML_CHECK_LAUNCH();
   return 0;
 }
 
-// The forms a product can run in, and what each costs in microseconds: `fixed` a tile (the epilogue), and a slice of 64
-// (KG of them) `alone` where a CU has one such workgroup at a time, `shared` times their number where it has more (the
-// L2's rate, or the matrix cores' for the largest). Measured over 1 to 16384 rows, K 256 to 8192, N 256 to 8192
-// (256 x 4096 x 4096: 32.2 / 24.1 / 20.1 us with KG 1 / 2 / 4; 1024 x 512 x 2048: 7.6 / 8.6 / 11.3; 16384 x 1024 x
-// 4096: 156 us in tiles of 256, 166 of 128; 6304 x 4096 x 1024: 94 and 57).
+// The tiled forms a product can run in, and what each costs in microseconds behind the launch: `fixed` a tile (its
+// ends), and a slice of 64 (KG of them) `alone` where a CU has one such workgroup at a time, `shared` times their
+// number where it has more (the L2's rate, or the matrix cores' for the largest). Measured over 1 to 16384 rows, K 256
+// to 8192, N 256 to 8192 (256 x 4096 x 4096: 32.2 / 24.1 / 20.1 us with KG 1 / 2 / 4; 1024 x 512 x 2048: 7.6 / 8.6 /
+// 11.3; 16384 x 1024 x 4096: 142 us in tiles of 256, 156 of 128; 6304 x 4096 x 1024: 94 and 57).
 struct Form {
   int bm, bn, kg, per_cu;
   double fixed, alone, shared;
 };
-constexpr Form kForms[] = {{64, 64, 1, 4, 1.0, 0.47, 0.25}, {64, 64, 2, 2, 1.5, 0.68, 0.5}, {64, 64, 4, 1, 2.5, 1.1, 1.1},
-                           {128, 128, 1, 2, 3.0, 0.65, 0.46}, {256, 256, 1, 1, 11.0, 1.6, 1.6}};
+constexpr Form kForms[] = {{64, 64, 1, 4, 1.0, 0.47, 0.25}, {64, 64, 2, 2, 1.0, 0.62, 0.5}, {64, 64, 4, 1, 1.5, 1.05, 1.05},
+                           {128, 128, 1, 2, 3.0, 0.65, 0.46}, {256, 256, 1, 1, 9.0, 1.6, 1.6}};
 
-static double cost(const DmlProductArgs* a, const Form& f) {
-  const double tiles = (double)row_tiles(a, f.bm) * ((a->N + f.bn - 1) / f.bn);
-  const long per = (long)((tiles + 255) / 256), rounds = per / f.per_cu, rest = per % f.per_cu;
+static long tiles_of(const DmlProductArgs* a, int bm, int bn) { return row_tiles(a, bm) * ((a->N + bn - 1) / bn); }
+
+static double cost(const DmlProductArgs* a, const Form& f, bool dma) {
+  const long per = (tiles_of(a, f.bm, f.bn) + 255) / 256, rounds = per / f.per_cu, rest = per % f.per_cu;
   const auto slice = [&](long n) { return n == 0 ? 0.0 : n * f.shared > f.alone ? n * f.shared : f.alone; };
   const int slices = (a->K + 64 * f.kg - 1) / (64 * f.kg);
-  return slices * (rounds * slice(f.per_cu) + slice(rest)) + per * f.fixed;
+  const double t = slices * (rounds * slice(f.per_cu) + slice(rest)) + per * f.fixed;
+  return dma ? t : 1.4 * t + (f.kg > 1 ? 2.5 : 0);  // through registers
 }
 
 template <class T>
@@ -581,17 +601,21 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   const bool dma = a->K % 8 == 0 && a->ldx % 8 == 0 && a->ldw % 8 == 0 && a->w_group % 8 == 0 &&
                    (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) &&
                    a->K < (1 << 28);
-  // product_rows: a column tile's weight in one pass, 3.5 us per 2048 of K and workgroup on a CU
-  const double tiles = (double)row_tiles(a, 16) * ((a->N + 15) / 16), k = a->K / 2048.0;
-  double least = (double)(long)((tiles + 255) / 256) * (k < 0.45 ? 0.45 : k) * 3.5 + 0.5;
-  int best = -1;
+  // product_rows in 16 x 16 (16 waves: 2048 of K in flight) and 32 x 32 (8 waves, 512): a workgroup on a CU takes 3.5 us
+  // per 2048 of K and 1.9 per 512 (17 x 3000 x 1000: 8.6 us, 500 x 500 x 500: 5.8, the best tile 12 and 8)
+  const double k = a->K / 2048.0;
+  const double rows16 = (tiles_of(a, 16, 16) + 255) / 256 * (k < 0.45 ? 0.45 : k) * 3.5 + 0.5;
+  const double rows32 = (tiles_of(a, 32, 32) + 255) / 256 * ((a->K + 511) / 512) * 1.9 + 1.0;
+  double least = rows16 < rows32 ? rows16 : rows32;
+  int best = rows16 < rows32 ? -1 : -2;
   for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
     if (!dma && (kForms[i].bm == 256 || kForms[i].kg == 2)) continue;  // not built through registers
-    const double c = cost(a, kForms[i]);
+    const double c = cost(a, kForms[i], dma);
     if (c < least) least = c, best = i;
   }
   switch (best) {
-    case -1: return launch_rows<T>(a, s);
+    case -2: return launch_rows<T, 2, 8, 1>(a, s);
+    case -1: return launch_rows<T, 1, 16, 2>(a, s);
     case 0: return dma ? launch<Tile<T, 64, 64, 2, 2, 1, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 1, false>>(a, s);
     case 1: return launch<Tile<T, 64, 64, 2, 2, 2, true>>(a, s);
     case 2: return dma ? launch<Tile<T, 64, 64, 2, 2, 4, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 4, false>>(a, s);
