@@ -110,14 +110,14 @@ struct Bias {
 };
 
 // A wave's accumulators (rows wm.., columns col0.., all of them inside) through the epilogue: of its 16 x 32 pieces
-// those whose number is `mine` modulo `of`. A lane has eight columns of a row in a piece. The residuals of four pieces
+// those whose number is `mine` modulo `of`. A lane has eight columns of a row in a piece. The residuals of G pieces
 // are read ahead of the stores, which could be to the same memory.
 template <int KIND, class C>
 __device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ],
                                           const Bias<C>& bias, int wm, int col0, int lane, int mine, int of) {
   typedef typename C::T T;
   const Act act = act_parameters(a.act);
-  constexpr int G = C::FJ < 4 ? C::FJ : 4;
+  constexpr int G = C::FJ % 4 == 0 ? 4 : C::FJ % 3 == 0 ? 3 : C::FJ % 2 == 0 ? 2 : 1;
   const int m0 = wm + (lane & 15);
 #pragma unroll
   for (int p = 0; p < C::FI / 2; ++p) {
@@ -577,21 +577,25 @@ static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
 // ends), and a slice of 64 (KG of them) `alone` where a CU has one such workgroup at a time, `shared` times their
 // number where it has more (the L2's rate, or the matrix cores' for the largest). Measured over 1 to 16384 rows, K 256
 // to 8192, N 256 to 8192 (256 x 4096 x 4096: 32.2 / 24.1 / 20.1 us with KG 1 / 2 / 4; 1024 x 512 x 2048: 7.6 / 8.6 /
-// 11.3; 16384 x 1024 x 4096: 142 us in tiles of 256, 156 of 128; 6304 x 4096 x 1024: 94 and 57).
+// 11.3; 17664 x 1024 x 4096: 192 us in tiles of 256, 160 of 192 x 128, 180 of 128; 16384 x 4096 x 4096: 430 / 462 /
+// 500; 6304 x 4096 x 1024: 83 / 76 / 54).
 struct Form {
   int bm, bn, kg, per_cu;
   double fixed, alone, shared;
 };
 constexpr Form kForms[] = {{64, 64, 1, 4, 1.0, 0.47, 0.25}, {64, 64, 2, 2, 1.0, 0.62, 0.5}, {64, 64, 4, 1, 1.5, 1.05, 1.05},
-                           {128, 128, 1, 2, 3.0, 0.65, 0.46}, {256, 256, 1, 1, 9.0, 1.6, 1.6}};
+                           {128, 128, 1, 2, 3.0, 0.65, 0.46}, {192, 128, 1, 2, 3.5, 0.81, 0.6}, {256, 256, 1, 1, 12.0, 1.6, 1.6}};
 
 static long tiles_of(const DmlProductArgs* a, int bm, int bn) { return row_tiles(a, bm) * ((a->N + bn - 1) / bn); }
 
 static double cost(const DmlProductArgs* a, const Form& f, bool dma) {
   const long per = (tiles_of(a, f.bm, f.bn) + 255) / 256, rounds = per / f.per_cu, rest = per % f.per_cu;
   const auto slice = [&](long n) { return n == 0 ? 0.0 : n * f.shared > f.alone ? n * f.shared : f.alone; };
+  // rows off the 128-byte lines: a slice takes two lines each, which costs the forms that the L2 bounds (5000 x 2000 x
+  // 6000 bf16: 134 us in tiles of 256, 153 of 192 x 128)
+  const double lines = f.bm < 256 && ((a->ldx | a->ldw) & 63) ? 1.2 : 1.0;
   const int slices = (a->K + 64 * f.kg - 1) / (64 * f.kg);
-  const double t = slices * (rounds * slice(f.per_cu) + slice(rest)) + per * f.fixed;
+  const double t = lines * slices * (rounds * slice(f.per_cu) + slice(rest)) + per * f.fixed;
   return dma ? t : 1.4 * t + (f.kg > 1 ? 2.5 : 0);  // through registers
 }
 
@@ -609,7 +613,7 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   double least = rows16 < rows32 ? rows16 : rows32;
   int best = rows16 < rows32 ? -1 : -2;
   for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
-    if (!dma && (kForms[i].bm == 256 || kForms[i].kg == 2)) continue;  // not built through registers
+    if (!dma && (kForms[i].bm > 128 || kForms[i].kg == 2)) continue;  // not built through registers
     const double c = cost(a, kForms[i], dma);
     if (c < least) least = c, best = i;
   }
@@ -620,6 +624,7 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
     case 1: return launch<Tile<T, 64, 64, 2, 2, 2, true>>(a, s);
     case 2: return dma ? launch<Tile<T, 64, 64, 2, 2, 4, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 4, false>>(a, s);
     case 3: return dma ? launch<Tile<T, 128, 128, 2, 2, 1, true>>(a, s) : launch<Tile<T, 128, 128, 2, 2, 1, false>>(a, s);
+    case 4: return launch<Tile<T, 192, 128, 2, 2, 1, true>>(a, s);
     default: return launch<Tile<T, 256, 256, 2, 4, 1, true>>(a, s);
   }
 }
