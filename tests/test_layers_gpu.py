@@ -93,7 +93,9 @@ NORM_SHAPES = [
     ((8, 197, 768), 32), ((2, 7, 7, 2048), 32), ((2, 9, 64), 1), ((5, 33, 66), 2), ((2, 3, 4, 5, 48), 16),
     ((2, 56, 56, 256), 32), ((1, 4096, 64), 64), ((3, 8), 2), ((1, 70000, 12), 3), ((40, 2, 40), 4),
     ((1, 73, 74, 2048), 32), ((2, 1000, 320), 32), ((1, 2, 8192), 1), ((2, 130, 130, 24), 2), ((700, 3, 32), 4),
-    ((2, 31, 33), 33), ((1, 28, 28, 1000), 8), ((64, 56, 56, 64), 32),
+    ((2, 31, 33), 33), ((1, 28, 28, 1000), 8), ((64, 56, 56, 64), 32), ((3, 100, 90), 5), ((2, 50, 99), 9),
+    ((2, 3000, 44), 1), ((4, 500, 60), 20), ((2, 70, 130), 10), ((1, 9000, 1000), 8), ((2, 40, 8200), 1), ((3, 20, 18), 2),
+    ((40, 28, 28, 512), 32), ((2, 12544, 64), 32), ((1, 40000, 48), 16),
 ]
 
 
