@@ -58,27 +58,33 @@ def _pitch(t: torch.Tensor, first: int, what: str) -> Tuple[int, int]:
 def _span(t: torch.Tensor) -> Tuple[int, int]:
     """First byte and the one behind the last of what t may touch."""
     p = t.data_ptr()
+    if t.is_contiguous():
+        return p, p + t.numel() * t.element_size()
     return p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def _apart(out: torch.Tensor, t: Optional[torch.Tensor], what: str, same: bool = False) -> None:
-    """out must share no memory with t: unless (same) it is t itself, or they are other columns of one buffer."""
-    if t is None or not out.numel() or not t.numel():
+def _apart(out: torch.Tensor, same: Optional[torch.Tensor], **others: Optional[torch.Tensor]) -> None:
+    """out must share no memory with the others unless they are other columns of one buffer; it may be `same` itself."""
+    if not out.numel():
         return
     a, b = _span(out)
-    c, d = _span(t)
-    if b <= c or d <= a:
-        return
-    if same and a == c and out.shape == t.shape and out.stride() == t.stride() and out.dtype == t.dtype:
-        return
-    steps = [s for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1]
-    if steps and out.element_size() == t.element_size() and out.stride() == t.stride() and out.shape[:-1] == t.shape[:-1]:
-        pitch = min(steps) * out.element_size()
-        gap = (c - a) % pitch  # t's columns begin here in out's rows
-        if abs(c - a) < pitch and gap >= out.shape[-1] * out.element_size() \
-                and gap + t.shape[-1] * t.element_size() <= pitch:
-            return
-    raise ValueError(f"out overlaps {what}")
+    for what, t in others.items():
+        if t is None or not t.numel():
+            continue
+        c, d = _span(t)
+        if b <= c or d <= a:
+            continue
+        if t is same and a == c and out.shape == t.shape and out.stride() == t.stride() and out.dtype == t.dtype:
+            continue
+        steps = [s for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1]
+        if steps and out.element_size() == t.element_size() and out.stride() == t.stride() \
+                and out.shape[:-1] == t.shape[:-1]:
+            pitch = min(steps) * out.element_size()
+            gap = (c - a) % pitch  # t's columns begin here in out's rows
+            if abs(c - a) < pitch and gap >= out.shape[-1] * out.element_size() \
+                    and gap + t.shape[-1] * t.element_size() <= pitch:
+                continue
+        raise ValueError(f"out overlaps {what}")
 
 
 def _vector(v: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, what: str) -> None:
@@ -155,14 +161,12 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         _, ldy = _pitch(out, 1, "out")
         if (rows > 1 and ldy < c) or (n > 1 and out.stride(0) < c):
             raise ValueError("out: its positions overlap each other")
-        _apart(out, x, "x", same=True)
-        _apart(out, weight, "weight")
-        _apart(out, bias, "bias")
+        _apart(out, x, x=x, weight=weight, bias=bias)
     if n > _INT or rows > _INT or n * groups > _INT:
         raise ValueError("x: over 2^31 - 1 samples, positions or groups")
     device = _ready(x, weight, bias, out)
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=x.dtype)
+        out = x.new_empty(shape)
     if not (n and rows):
         return out
     weight, bias = _f32(weight), _f32(bias)
@@ -213,17 +217,13 @@ def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, wha
         ldy = _pitch(out, 0, "out")[1]
         if m > 1 and ldy < n:
             raise ValueError("out: its rows overlap each other")
-        _apart(out, x, "x")
-        _apart(out, weight, "weight")
-        _apart(out, bias, "bias")
-        _apart(out, ends, "ends")
-        _apart(out, residual, "residual", same=True)
+        _apart(out, residual, x=x, weight=weight, bias=bias, ends=ends, residual=residual)
     if max(m, n, k, e) > _INT - 512:
         raise ValueError(f"{what}: a dimension over 2^31 - 513")
     device = _ready(x, weight, ends, bias, residual, out)
     fill = 0
     if out is None:
-        out = torch.empty(shape, device=x.device, dtype=to)
+        out = x.new_empty(shape, dtype=to)
         fill = int(ends is not None)
     if not (m and n):
         return out
