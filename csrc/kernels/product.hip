@@ -604,7 +604,7 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   // LDS-DMA moves aligned 16 bytes at 32-bit offsets from a tile's first row
   const bool dma = a->K % 8 == 0 && a->ldx % 8 == 0 && a->ldw % 8 == 0 && a->w_group % 8 == 0 &&
                    (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) &&
-                   a->K < (1 << 28);
+                   255 * (a->ldx > a->ldw ? a->ldx : a->ldw) + a->K < (1 << 30) - 512;
   // product_rows in 16 x 16 (16 waves: 2048 of K in flight) and 32 x 32 (8 waves, 512): a workgroup on a CU takes 3.5 us
   // per 2048 of K and 1.9 per 512 (17 x 3000 x 1000: 8.6 us, 500 x 500 x 500: 5.8, the best tile 12 and 8)
   const double k = a->K / 2048.0;
@@ -633,8 +633,9 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
 }  // namespace dml
 
 extern "C" int dml_product(const DmlProductArgs* a, hipStream_t s) {
-  if (!a || a->M < 0 || a->N < 0 || a->K < 0 || a->E < 0 || (!a->ends && a->E != 1)) {
-    dml_set_error("dml_product: need M, N, K, E >= 0, and E = 1 without ends");
+  if (!a || a->M < 0 || a->N < 0 || a->K < 0 || a->E < 0 || a->K > (1 << 30) || a->M > INT_MAX - 512 ||
+      a->N > INT_MAX - 512 || a->E > INT_MAX - 512 || (!a->ends && a->E != 1)) {
+    dml_set_error("dml_product: need M, N, K, E from 0 to 2^31 - 513, K to 2^30, and E = 1 without ends");
     return -1;
   }
   if ((a->dtype != DML_BF16 && a->dtype != DML_F16) || a->act < 0 || a->act >= DML_ACT_COUNT) {
@@ -643,7 +644,8 @@ extern "C" int dml_product(const DmlProductArgs* a, hipStream_t s) {
   }
   if (a->M == 0 || a->N == 0) return 0;
   if (!a->y || (a->K > 0 && a->E > 0 && (!a->x || !a->w)) || a->ldy < a->N || a->ldx < 0 || a->ldw < 0 ||
-      a->ldr < 0) {
+      a->ldr < 0 || a->w_group < 0 || a->bias_group < 0 || a->ldx > INT64_MAX / 4 / a->M || a->ldw > INT64_MAX / 4 / a->N ||
+      a->ldy > INT64_MAX / 4 / a->M || a->ldr > INT64_MAX / 4 / a->M) {
     dml_set_error("dml_product: null tensor or row stride out of range");
     return -1;
   }

@@ -162,8 +162,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         if (rows > 1 and ldy < c) or (n > 1 and out.stride(0) < c):
             raise ValueError("out: its positions overlap each other")
         _apart(out, x, x=x, weight=weight, bias=bias)
-    if n > _INT or rows > _INT or n * groups > _INT:
-        raise ValueError("x: over 2^31 - 1 samples, positions or groups")
+    if max(n, rows, c, n * groups) > _INT:
+        raise ValueError("x: over 2^31 - 1 samples, positions, channels or groups")
     device = _ready(x, weight, bias, out)
     if out is None:
         out = x.new_empty(shape)
@@ -218,8 +218,8 @@ def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, wha
         if m > 1 and ldy < n:
             raise ValueError("out: its rows overlap each other")
         _apart(out, residual, x=x, weight=weight, bias=bias, ends=ends, residual=residual)
-    if max(m, n, k, e) > _INT - 512:
-        raise ValueError(f"{what}: a dimension over 2^31 - 513")
+    if max(m, n, e) > _INT - 512 or k > 2 ** 30:
+        raise ValueError(f"{what}: a dimension over 2^31 - 513, or K over 2^30")
     device = _ready(x, weight, ends, bias, residual, out)
     fill = 0
     if out is None:

@@ -1,4 +1,6 @@
 """Arguments that ops.group_norm, ops.linear and ops.grouped_linear refuse, before anything reaches a device."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -111,3 +113,47 @@ def test_argument_structs_match_the_library():
     """lib() compares the struct sizes; the new ones are among those compared."""
     assert {"GroupNormArgs", "ProductArgs"} <= set(N.ABI_STRUCTS)
     N.lib()
+
+
+def _norm_args(**kw):
+    d = {"x": 16, "y": 16, "weight": 0, "bias": 0, "xn": 64, "yn": 64, "ldx": 16, "ldy": 16, "ws": 0, "ws_bytes": 0,
+         "N": 1, "HW": 4, "C": 16, "G": 4, "dtype": 0, "act": 0, "eps": 1e-5, **kw}
+    return C.byref(N.GroupNormArgs(*d.values()))
+
+
+@pytest.mark.parametrize("kw", [{"C": 0}, {"G": 0}, {"G": 3}, {"N": -1}, {"HW": -1}, {"dtype": 3}, {"dtype": -1},
+                                {"act": 5}, {"act": -1}, {"x": None}, {"y": None}, {"ldy": 15}, {"ldx": -1}])
+def test_library_refuses_group_norm(kw):
+    """The library's own checks: nothing is launched, the reason is left for dml_last_error."""
+    assert N.lib().dml_group_norm(_norm_args(**kw), None) == -1
+    assert N.lib().dml_last_error().startswith(b"dml_group_norm")
+
+
+def test_library_group_norm_asks_for_its_workspace():
+    """A sample too long for one workgroup: the size comes back, and nothing is launched without it."""
+    need = N.lib().dml_group_norm(_norm_args(HW=200000, xn=3200000, yn=3200000), None)
+    assert need > 0 and need % 8 == 0
+    assert N.lib().dml_group_norm(_norm_args(HW=200000, xn=3200000, yn=3200000, ws=16, ws_bytes=need - 1), None) == need
+    assert N.lib().dml_group_norm(_norm_args(N=0), None) == 0
+    assert N.lib().dml_group_norm(None, None) == -1
+
+
+def _prod_args(**kw):
+    d = {"x": 16, "w": 16, "bias": 0, "res": 0, "y": 16, "ends": 0, "ldx": 8, "ldw": 8, "w_group": 0, "bias_group": 0,
+         "ldr": 0, "ldy": 8, "M": 4, "N": 8, "K": 8, "E": 1, "dtype": 0, "out_f32": 0, "act": 0, "act_last": 0,
+         "ends64": 0, "fill": 0, **kw}
+    return C.byref(N.ProductArgs(*d.values()))
+
+
+@pytest.mark.parametrize("kw", [{"M": -1}, {"N": -1}, {"K": -1}, {"E": -1}, {"E": 2}, {"K": 2 ** 30 + 1}, {"M": 2 ** 31 - 1},
+                                {"dtype": 2}, {"dtype": -1}, {"act": 5}, {"x": None}, {"w": None}, {"y": None}, {"ldy": 7},
+                                {"ldx": -1}, {"ldw": -8}, {"ldr": -1}, {"w_group": -1}, {"ldx": 2 ** 62}, {"ldy": 2 ** 62}])
+def test_library_refuses_product(kw):
+    assert N.lib().dml_product(_prod_args(**kw), None) == -1
+    assert N.lib().dml_last_error().startswith(b"dml_product")
+
+
+def test_library_product_of_nothing():
+    assert N.lib().dml_product(_prod_args(M=0), None) == 0
+    assert N.lib().dml_product(_prod_args(N=0), None) == 0
+    assert N.lib().dml_product(None, None) == -1

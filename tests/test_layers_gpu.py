@@ -511,3 +511,46 @@ def test_repeats_are_bit_identical():
     want = (ops.linear(x, w, b), ops.group_norm(img, 6))
     for _ in range(5):
         assert torch.equal(ops.linear(x, w, b), want[0]) and torch.equal(ops.group_norm(img, 6), want[1])
+
+
+@pytest.mark.parametrize("step", (0, 1, 2, 8, 24))
+@pytest.mark.parametrize("m, k, n", [(5, 96, 40), (300, 96, 136), (400, 1024, 256)])
+def test_linear_rows_that_share_memory(m, k, n, step):
+    """Rows closer than they are long (windows over one sequence), and one row for all."""
+    g = gen(67)
+    buf = normal(g, m * max(step, 1) + k).to(BF)
+    _, w, b = operands(g, 1, k, n, BF)
+    check_linear(buf.as_strided((m, k), (step, 1)), w, b, "relu")
+    check_linear(normal(g, m, k).to(BF), w[:1].expand(n, k), None)
+
+
+def test_grouped_linear_shared_weight_and_many_groups():
+    g = gen(71)
+    x, w, b = operands(g, 600, 64, 96, BF)
+    ends = torch.tensor([100, 350, 600], device="cuda", dtype=torch.int32)
+    y, v, err = rows64(x, w, b, None, "none", False)
+    close(ops.grouped_linear(x, w.expand(3, 96, 64), ends, b.expand(3, 96)), y, err, v)
+    check_grouped(g, [0, 1, 2, 0, 0, 3] * 170, 32, 48, BF, "relu", spare=5)
+
+
+@pytest.mark.parametrize("m, k, n", [(70000, 8, 16), (40000, 136, 24), (3, 40000, 64), (20, 16, 30000), (66000, 64, 1)])
+def test_linear_long_and_thin(m, k, n):
+    g = gen(73)
+    x, w, b = operands(g, m, k, n, BF)
+    check_linear(x, w, b, "silu")
+
+
+def test_calls_on_a_side_stream_follow_its_order():
+    """Inputs made on a side stream just ahead of the calls there, results used there just behind them."""
+    g = gen(79)
+    x, w, b = operands(g, 2000, 1024, 512, BF)
+    img = normal(g, 4, 9000, 64).to(BF)
+    want = (ops.linear(2 * x, w, b, act="gelu"), ops.group_norm(3 * img, 8, act="silu"))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            y = ops.linear(2 * x, w, b, act="gelu") + 0
+            z = ops.group_norm(3 * img, 8, act="silu") + 0
+        side.synchronize()
+        assert torch.equal(y, want[0]) and torch.equal(z, want[1])
