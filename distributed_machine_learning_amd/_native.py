@@ -216,8 +216,10 @@ def _check_abi(L) -> None:
         return
     n = len(ABI_STRUCTS)
     out = (C.c_int * n)()
-    f(out, n)
-    for i, name in enumerate(ABI_STRUCTS):
+    known = f(out, n)
+    if known < n and not os.environ.get("DML_LIB"):  # an older variant library has the first of them
+        raise NativeError(f"ABI mismatch: the library has {known} argument structs, _native.py {n}")
+    for i, name in enumerate(ABI_STRUCTS[:known]):
         want = C.sizeof(globals()[name])
         if out[i] != want:
             raise NativeError(f"ABI mismatch: sizeof(Dml{name}) = {out[i]} in the library, {want} in _native.py")
