@@ -552,8 +552,8 @@ static long row_tiles(const DmlProductArgs* a, int bm) {
 template <class C>
 static int launch(const DmlProductArgs* a, hipStream_t s) {
   const long blocks = row_tiles(a, C::BM) * ((a->N + C::BN - 1) / C::BN);
-  if (blocks > INT_MAX) {
-    dml_set_error("dml_product: over 2^31 tiles");
+  if (blocks > (long)(UINT_MAX / C::NT)) {
+    dml_set_error("dml_product: over 2^32 threads");
     return -1;
   }
   hipLaunchKernelGGL(product_tile<C>, dim3((unsigned)blocks), dim3(C::NT), 0, s, *a);
@@ -564,8 +564,8 @@ static int launch(const DmlProductArgs* a, hipStream_t s) {
 template <class T, int F, int NW, int U>
 static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
   const long blocks = row_tiles(a, 16 * F) * ((a->N + 16 * F - 1) / (16 * F));
-  if (blocks > INT_MAX) {
-    dml_set_error("dml_product: over 2^31 tiles");
+  if (blocks > (long)(UINT_MAX / (NW * 64))) {
+    dml_set_error("dml_product: over 2^32 threads");
     return -1;
   }
   hipLaunchKernelGGL((product_rows<T, F, F, NW, U>), dim3((unsigned)blocks), dim3(NW * 64), 0, s, *a);
@@ -604,7 +604,7 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   // LDS-DMA moves aligned 16 bytes at 32-bit offsets from a tile's first row
   const bool dma = a->K % 8 == 0 && a->ldx % 8 == 0 && a->ldw % 8 == 0 && a->w_group % 8 == 0 &&
                    (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) &&
-                   255 * (a->ldx > a->ldw ? a->ldx : a->ldw) + a->K < (1 << 30) - 512;
+                   255 * (a->ldx > a->ldw ? a->ldx : a->ldw) + a->K < (1 << 30) - 512 && a->K < (1 << 22);
   // product_rows in 16 x 16 (16 waves: 2048 of K in flight) and 32 x 32 (8 waves, 512): a workgroup on a CU takes 3.5 us
   // per 2048 of K and 1.9 per 512 (17 x 3000 x 1000: 8.6 us, 500 x 500 x 500: 5.8, the best tile 12 and 8)
   const double k = a->K / 2048.0;
