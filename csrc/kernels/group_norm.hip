@@ -13,12 +13,14 @@
 //    its one write: up to 400 KiB in a workgroup.
 //  * stats + apply: slabs beyond that, or too few slabs to fill the card. Every chunk of rows
 //    yields (mean, sum of squared distances from it) per group in the workspace; the second
-//    kernel merges the chunks and reads x again.
+//    kernel merges the chunks and reads x again. Between them, where there are many chunks,
+//    `join` merges each group's once for all.
 //
 // Statistics in fp32 from centred values (E[x^2] - mu^2 loses all digits where the mean is
 // large against the spread), chunks merged by the parallel form of the same
 // (M2 = sum M2_i + n_i (mu_i - mu)^2), all sums in a fixed order.
 #include "activation.h"
+#include <climits>
 
 namespace dml {
 namespace gn {
@@ -28,6 +30,13 @@ constexpr int kMaxGroups = 256;  // groups of a slab
 
 // t / d for 0 <= t < 2^21: t + 1/2 is at least 1/(2d) away from a multiple of d, the reciprocal's error below that
 __device__ __forceinline__ int div_small(int t, float inv) { return (int)(((float)t + 0.5f) * inv); }
+
+// The instruction takes no subnormals: those go through it 2^64 times as large.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const bool tiny = v < 0x1p-100f;
+  const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p64f : v);
+  return tiny ? r * 0x1p32f : r;
+}
 
 // How a slab of S >= V channels lies over NT threads.
 template <class T, int NT, bool CH>
@@ -281,7 +290,7 @@ __global__ __launch_bounds__(NT) void one_pass(DmlGroupNormArgs a, int S, int on
   s.mine(stat + kMaxGroups, var);
   const float inv = 1.f / ((float)a.HW * (float)s.cg);
 #pragma unroll
-  for (int p = 0; p < PC; ++p) var[p] = __builtin_amdgcn_rsqf(var[p] * inv + a.eps);
+  for (int p = 0; p < PC; ++p) var[p] = inv_sqrt(var[p] * inv + a.eps);
 #pragma unroll
   for (int j = 0; j < V; ++j) f.scale[j] *= var[PC == 1 ? 0 : j];
   T* y = (T*)a.y + n * a.yn + c + s.rt * a.ldy;
@@ -307,8 +316,44 @@ __global__ __launch_bounds__(NT) void stats(DmlGroupNormArgs a, int S, int rows,
     ((float2*)a.ws)[((int64_t)n * a.G + slab * s.gs + g) * chunks + chunk] = make_float2(stat[g], stat[kMaxGroups + g]);
 }
 
+// All rows' (mean, M2) of a group from its `parts` of `rows` rows each, by L lanes of a wave: every lane has it.
+template <int L>
+__device__ __forceinline__ float2 joined(const float2* ws, int parts, int rows, int HW, int cg, int lane) {
+  float sum = 0.f, m2 = 0.f;
+#pragma unroll 4
+  for (int i = lane; i < parts; i += L) sum += ws[i].x * (float)(min(rows, HW - i * rows) * cg);
+  const float mu = over_lanes<L>(sum) / ((float)HW * (float)cg);
+#pragma unroll 4
+  for (int i = lane; i < parts; i += L) {
+    const float d = ws[i].x - mu;
+    m2 += ws[i].y + d * d * (float)(min(rows, HW - i * rows) * cg);
+  }
+  return make_float2(mu, over_lanes<L>(m2));
+}
+
+// Long samples: a group's chunks joined once, and not in each of the chunks' workgroups again (chunks^2 pairs to
+// read). Wave w of a group's workgroup joins every 16th run of chunks, its first thread the 16 results.
+template <int NT>
+__global__ __launch_bounds__(NT) void join(DmlGroupNormArgs a, int rows, int chunks) {
+  __shared__ float2 part[NT / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = (chunks + NT / 64 - 1) / (NT / 64), first = min(wave * per, chunks), n = min(per, chunks - first);
+  const float2* ws = (const float2*)a.ws + (int64_t)blockIdx.x * chunks + first;
+  const int cg = a.C / a.G, span = per * rows;
+  const float2 mine = n > 0 ? joined<64>(ws, n, rows, min(span, a.HW - first * rows), cg, lane) : make_float2(0.f, 0.f);
+  if (lane == 0) part[wave] = mine;
+  __syncthreads();
+  if (wave == 0) {
+    const int parts = (chunks + per - 1) / per;
+    const float2 all = joined<64>(part, parts, span, a.HW, cg, lane);
+    if (lane == 0) ((float2*)a.ws)[(int64_t)a.N * a.G * chunks + blockIdx.x] = all;
+  }
+}
+
+// ws: the groups' pairs, `parts` of `part_rows` rows each
 template <class T, int NT, int R, bool CH>
-__global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows, int chunks) {
+__global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows, int chunks, const float2* ws, int parts,
+                                            int part_rows) {
   typedef Slab<T, NT, CH> SL;
   constexpr int V = SL::V, PC = SL::PC;
   __shared__ float stat[2 * kMaxGroups];
@@ -321,21 +366,10 @@ __global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows,
   const float total = (float)a.HW * (float)s.cg;
   each_group<NT>(s.gs, [&](int g, int lane, auto lanes) {
     constexpr int L = decltype(lanes)::value;
-    const float2* ws = (const float2*)a.ws + ((int64_t)n * a.G + slab * s.gs + g) * chunks;
-    float sum = 0.f, m2 = 0.f;
-#pragma unroll 4
-    for (int i = lane; i < chunks; i += L) sum += ws[i].x * (float)(min(rows, a.HW - i * rows) * s.cg);
-    sum = over_lanes<L>(sum);
-    const float mu = sum / total;
-#pragma unroll 4
-    for (int i = lane; i < chunks; i += L) {
-      const float d = ws[i].x - mu;
-      m2 += ws[i].y + d * d * (float)(min(rows, a.HW - i * rows) * s.cg);
-    }
-    m2 = over_lanes<L>(m2);
+    const float2 all = joined<L>(ws + ((int64_t)n * a.G + slab * s.gs + g) * parts, parts, part_rows, a.HW, s.cg, lane);
     if (lane == 0) {
-      stat[g] = mu;
-      stat[kMaxGroups + g] = 1.f / sqrtf(m2 / total + a.eps);
+      stat[g] = all.x;
+      stat[kMaxGroups + g] = inv_sqrt(all.y / total + a.eps);
     }
   });
   const int c = slab * S + s.c, row0 = chunk * rows, mine = min(rows, a.HW - row0);
@@ -348,6 +382,7 @@ __global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows,
     if (i < count) h.v[i].load(x + (int64_t)(s.rt + i * s.RT) * a.ldx);
   Affine<T, PC> f;
   f.load(a, c);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // y may be x, and a slab's last two vectors may share channels
   __syncthreads();
   if (!s.on) return;
   s.mine(stat, f.mu);
@@ -385,7 +420,7 @@ __global__ __launch_bounds__(256) void by_element(DmlGroupNormArgs a) {
     const float d = to_f32(x[(i / cg) * a.ldx + i % cg]) - mu;
     s += d * d;
   }
-  const float rs = 1.f / sqrtf(total(s) / (float)count + a.eps);
+  const float rs = inv_sqrt(total(s) / (float)count + a.eps);
   for (int64_t i = threadIdx.x; i < count; i += 256) {
     const int c = (int)(i % cg);
     const float v = (to_f32(x[(i / cg) * a.ldx + c]) - mu) * (rs * (a.weight ? a.weight[c0 + c] : 1.f)) +
@@ -399,7 +434,7 @@ __global__ __launch_bounds__(256) void by_element(DmlGroupNormArgs a) {
 enum { ONE_PASS, SPLIT, ELEMENTS };
 struct Plan {
   int mode, S, shape, rows, chunks, once;
-  bool ch;
+  bool ch, join;
 };
 
 // one_pass forms: threads, vectors in registers and in LDS. 14 vectors a thread leave two 512-thread or four 256-thread
@@ -455,6 +490,9 @@ static Plan plan(const DmlGroupNormArgs* a) {
   // loads marked as not read again where x is beyond the caches anyway and a pixel's run is most of a line (256 x 784 x
   // 512 bf16: 92 -> 82 us; with runs of 32 bytes 15 % slower, and smaller inputs are often still cached)
   p.once = bytes / 2 >= 96e6 && p.S * es >= 64;
+  // 2^22 pairs are where joining each group first is worth its launch (1 x 65536 x 512 in 256 chunks: 39.5 us without,
+  // 42.5 with; 8 x 65536 x 256: 178 and 159; 1 x 1048576 x 64 in 4096: 261 and 69)
+  p.join = p.mode == SPLIT && p.chunks >= 256 && (double)a->N * a->G * p.chunks * p.chunks >= 4194304.0;
   if (best == 1e30) p.mode = ELEMENTS;
   return p;
 }
@@ -471,8 +509,14 @@ static void launch_one(const DmlGroupNormArgs* a, const Plan& p, dim3 grid, hipS
 
 template <class T, int NT, int R, bool CH>
 static void launch_split(const DmlGroupNormArgs* a, const Plan& p, dim3 grid, hipStream_t s) {
+  const float2* ws = (const float2*)a->ws;
   hipLaunchKernelGGL((stats<T, NT, R, CH>), grid, dim3(NT), 0, s, *a, p.S, p.rows, p.chunks);
-  hipLaunchKernelGGL((apply<T, NT, R, CH>), grid, dim3(NT), 0, s, *a, p.S, p.rows, p.chunks);
+  if (p.join) {
+    hipLaunchKernelGGL(join<1024>, dim3((unsigned)a->N * a->G), dim3(1024), 0, s, *a, p.rows, p.chunks);
+    ws += (int64_t)a->N * a->G * p.chunks;
+  }
+  hipLaunchKernelGGL((apply<T, NT, R, CH>), grid, dim3(NT), 0, s, *a, p.S, p.rows, p.chunks, ws, p.join ? 1 : p.chunks,
+                     p.join ? a->HW : p.rows);
 }
 
 template <class T, bool CH>
@@ -494,8 +538,8 @@ static int launch(const DmlGroupNormArgs* a, const Plan& p, hipStream_t s) {
 }
 
 static int check(const DmlGroupNormArgs* a) {
-  if (!a || a->N < 0 || a->HW < 0 || a->C < 1 || a->G < 1 || a->C % a->G) {
-    dml_set_error("dml_group_norm: need N, HW >= 0 and a channel count that the groups divide");
+  if (!a || a->N < 0 || a->HW < 0 || a->HW > INT_MAX - 4096 || a->C < 1 || a->G < 1 || a->C % a->G) {
+    dml_set_error("dml_group_norm: need N >= 0, HW from 0 to 2^31 - 4097 and a channel count that the groups divide");
     return -1;
   }
   if (a->dtype < DML_BF16 || a->dtype > DML_F32 || a->act < 0 || a->act >= DML_ACT_COUNT) {
@@ -518,11 +562,13 @@ extern "C" int64_t dml_group_norm(const DmlGroupNormArgs* a, hipStream_t s) {
   if (a->N == 0 || a->HW == 0) return 0;
   const Plan p = plan(a);
   const long per = (long)a->N * (p.mode == ELEMENTS ? a->G : a->C / p.S);
-  if (per > 0x7fffffffl || (p.mode == SPLIT && per > 0x7fffffffl / p.chunks)) {
-    dml_set_error("dml_group_norm: over 2^31 workgroups");
+  // a grid has under 2^32 threads
+  const long most = UINT_MAX / (p.mode == ELEMENTS ? 256 : p.mode == ONE_PASS ? kShapes[p.shape][0] : p.shape == 2 ? 1024 : 256);
+  if (per > (p.mode == SPLIT ? most / p.chunks : most) || (p.join && (long)a->N * a->G > UINT_MAX / 1024)) {
+    dml_set_error("dml_group_norm: over 2^32 threads");
     return -1;
   }
-  const int64_t need = p.mode == SPLIT ? (int64_t)a->N * a->G * p.chunks * 8 : 0;
+  const int64_t need = p.mode == SPLIT ? (int64_t)a->N * a->G * (p.chunks + p.join) * 8 : 0;
   if (need > a->ws_bytes || (need && !a->ws)) return need;
   switch (a->dtype) {
     case DML_BF16: return p.ch ? launch<bf16, true>(a, p, s) : launch<bf16, false>(a, p, s);

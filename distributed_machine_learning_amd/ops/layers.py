@@ -146,8 +146,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     n, c = shape[0], shape[-1]
     if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or c < 1 or c % groups:
         raise ValueError(f"groups must divide the {c} channels, got {groups!r}")
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative, got {eps}")
+    if not 0 <= eps <= 3e38:
+        raise ValueError(f"eps must be a number from 0 to 3e38, got {eps}")
     if weight is not None:
         _vector(weight, (c,), x.dtype, "weight")
     if bias is not None:
@@ -162,8 +162,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         if (rows > 1 and ldy < c) or (n > 1 and out.stride(0) < c):
             raise ValueError("out: its positions overlap each other")
         _apart(out, x, x=x, weight=weight, bias=bias)
-    if max(n, rows, c, n * groups) > _INT:
-        raise ValueError("x: over 2^31 - 1 samples, positions, channels or groups")
+    if max(n, rows, c, n * groups) > _INT - 4096:
+        raise ValueError("x: over 2^31 - 4097 samples, positions, channels or groups")
     device = _ready(x, weight, bias, out)
     if out is None:
         out = x.new_empty(shape)

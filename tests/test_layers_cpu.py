@@ -32,6 +32,7 @@ BUF = torch.zeros(4, 64, dtype=BF)
     (ValueError, "groups must divide", lambda: _norm(_t(2, 3, 0))),
     (ValueError, "eps", lambda: _norm(eps=-1e-5)),
     (ValueError, "eps", lambda: _norm(eps=float("nan"))),
+    (ValueError, "eps", lambda: _norm(eps=1e39)),
     (ValueError, "weight: expected shape", lambda: _norm(weight=_t(8))),
     (TypeError, "bias: expected", lambda: _norm(bias=_t(16, dtype=torch.float16))),
     (ValueError, "last dimension", lambda: _norm(_t(2, 16, 9).transpose(1, 2))),
@@ -122,7 +123,8 @@ def _norm_args(**kw):
 
 
 @pytest.mark.parametrize("kw", [{"C": 0}, {"G": 0}, {"G": 3}, {"N": -1}, {"HW": -1}, {"dtype": 3}, {"dtype": -1},
-                                {"act": 5}, {"act": -1}, {"x": None}, {"y": None}, {"ldy": 15}, {"ldx": -1}])
+                                {"act": 5}, {"act": -1}, {"x": None}, {"y": None}, {"ldy": 15}, {"ldx": -1},
+                                {"HW": 2 ** 31 - 1}, {"N": 2 ** 25, "HW": 1, "C": 3, "G": 3}])
 def test_library_refuses_group_norm(kw):
     """The library's own checks: nothing is launched, the reason is left for dml_last_error."""
     assert N.lib().dml_group_norm(_norm_args(**kw), None) == -1
@@ -147,7 +149,8 @@ def _prod_args(**kw):
 
 @pytest.mark.parametrize("kw", [{"M": -1}, {"N": -1}, {"K": -1}, {"E": -1}, {"E": 2}, {"K": 2 ** 30 + 1}, {"M": 2 ** 31 - 1},
                                 {"dtype": 2}, {"dtype": -1}, {"act": 5}, {"x": None}, {"w": None}, {"y": None}, {"ldy": 7},
-                                {"ldx": -1}, {"ldw": -8}, {"ldr": -1}, {"w_group": -1}, {"ldx": 2 ** 62}, {"ldy": 2 ** 62}])
+                                {"ldx": -1}, {"ldw": -8}, {"ldr": -1}, {"w_group": -1}, {"ldx": 2 ** 62}, {"ldy": 2 ** 62},
+                                {"M": 2 ** 31 - 600, "N": 2 ** 20, "ldy": 2 ** 20}])
 def test_library_refuses_product(kw):
     assert N.lib().dml_product(_prod_args(**kw), None) == -1
     assert N.lib().dml_last_error().startswith(b"dml_product")

@@ -55,19 +55,28 @@ def normal(g, *shape):
 # ---------------------------------------------------------------- group norm
 
 
+def over(t, f):
+    """f (torch.sum, or torch.amax of magnitudes) over the positions and a group's channels of t [n, L, G, cg], 512
+    positions at a time first: torch's own reductions of many values to a few have come out wrong on the device, now
+    and then and by a lot, where its CPU's and these agree."""
+    n, l, g, cg = t.shape
+    t = torch.nn.functional.pad(t, (0, 0, 0, 0, 0, -l % 512)).reshape(n, -1, 512, g, cg)
+    return f(f(t, 2), (1, 3)).reshape(n, 1, g, 1)
+
+
 def norm64(x, groups, weight, bias, eps, act):
     """(y, v, err): the formula in 64 bits, its value before the activation, and how far fp32 may be off."""
     n, c = x.shape[0], x.shape[-1]
     xd = x.double().reshape(n, -1, groups, c // groups)
     count = xd.shape[1] * xd.shape[3]
-    mu = xd.mean((1, 3), keepdim=True)
-    var = (xd - mu).square().mean((1, 3), keepdim=True)
+    mu = over(xd, torch.sum) / count
+    var = over((xd - mu).square(), torch.sum) / count
     rs = 1 / torch.sqrt(var + eps)
     d = (count / 64 + 64) * U
     # |mu' - mu| <= d mean|x|; the centred values carry that and a step of x; the variance carries their square
-    emu = d * xd.abs().mean((1, 3), keepdim=True)
+    emu = d * over(xd.abs(), torch.sum) / count
     ec = emu + U * (xd.abs() + mu.abs())
-    evar = d * (var + emu ** 2) + emu ** 2 + 2 * U * xd.abs().amax((1, 3), keepdim=True) * var.sqrt()
+    evar = d * (var + emu ** 2) + emu ** 2 + 2 * U * over(xd.abs(), torch.amax) * var.sqrt()
     # the relative error of 1/sqrt(var + eps), which stays below 1/sqrt(eps) however far var is off
     rel = (evar / (var + eps)).clamp(max=1) + 4 * U
     xhat = (xd - mu) * rs
@@ -162,6 +171,33 @@ def test_group_norm_keeps_bad_values_to_their_group(shape, groups, bad):
     hit[1, :, per:2 * per] = True
     assert y[hit].isnan().all() and torch.equal(y[~hit], want[~hit])
     assert ops.group_norm(x, groups, act="relu")[hit].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", (BF, FP))
+@pytest.mark.parametrize("shape, groups", [((1, 300000, 64), 8), ((2, 70001, 256), 32), ((1, 400000, 35), 5),
+                                           ((1, 1000, 1000, 24), 3), ((1, 150000, 520), 520)])
+def test_group_norm_long_samples(shape, groups, dtype):
+    """Hundreds of chunks to a group, also in place, where neighbouring lanes share a slab's last channels."""
+    g = gen(23)
+    c = shape[-1]
+    x = (2 * normal(g, *shape) + normal(g, c)).to(dtype)
+    w, b = 1 + 0.2 * normal(g, c), 0.2 * normal(g, c)
+    want = check_norm(x, groups, w, b, act="silu")
+    for _ in range(3):
+        y = x.clone()
+        assert ops.group_norm(y, groups, w, b, act="silu", out=y) is y and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("shape, groups", [((2, 50, 64), 8), ((1, 9000, 96), 3), ((2, 20, 35), 5), ((2, 9, 3), 3)])
+def test_group_norm_of_tiny_values(shape, groups):
+    """Variances of 2^-132: subnormal in fp32, where a square is off by up to 2^-150, so 2^-18 of the variance. That
+    four times (squares, two levels of merging, the mean) is 2 x 2^-18 of the result."""
+    x = normal(gen(29), *shape) * 2.0 ** -66
+    y, _, err = norm64(x, groups, None, None, 0.0, "none")
+    xd = x.double().reshape(shape[0], -1, groups, shape[-1] // groups)
+    count = xd.shape[1] * xd.shape[3]
+    var = over((xd - over(xd, torch.sum) / count).square(), torch.sum) / count
+    close(ops.group_norm(x, groups, eps=0.0), y, err + 2 * 2.0 ** -18 * y.abs() * (2.0 ** -132 / var.min()))
 
 
 def test_group_norm_empty():
@@ -538,6 +574,15 @@ def test_linear_long_and_thin(m, k, n):
     g = gen(73)
     x, w, b = operands(g, m, k, n, BF)
     check_linear(x, w, b, "silu")
+
+
+def test_linear_longest_rows():
+    """K at the limit of 32-bit byte offsets, in shared rows: three products that are not zero, so an exact sum."""
+    k = 2 ** 30 - 520
+    x, w = (torch.zeros(k, device="cuda", dtype=BF) for _ in range(2))
+    for i, v in ((0, 1.0), (k // 2 + 3, 2.0), (k - 1, 4.0)):
+        x[i], w[i] = v, 1.0
+    assert (ops.linear(x.expand(2, k), w.expand(3, k)) == 7).all()
 
 
 def test_calls_on_a_side_stream_follow_its_order():
