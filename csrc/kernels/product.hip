@@ -109,9 +109,9 @@ struct Bias {
   }
 };
 
-// A wave's accumulators (rows wm.., columns col0.., all of them inside) through the epilogue: of its 16 x 32 pieces
-// those whose number is `mine` modulo `of`. A lane has eight columns of a row in a piece. The residuals of G pieces
-// are read ahead of the stores, which could be to the same memory.
+// A wave's accumulators (rows wm.., columns col0..) through the epilogue: of its 16 x 32 pieces those whose number is
+// `mine` modulo `of`. A lane has eight columns of a row in a piece, and leaves them out unless all are inside. The
+// residuals of G pieces are read ahead of the stores, which could be to the same memory.
 template <int KIND, class C>
 __device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ],
                                           const Bias<C>& bias, int wm, int col0, int lane, int mine, int of) {
@@ -122,6 +122,7 @@ __device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& 
 #pragma unroll
   for (int p = 0; p < C::FI / 2; ++p) {
     const int64_t col = col0 + p * 32 + (lane >> 4) * 8;
+    if (col + 8 > a.N) continue;
     const int64_t y0 = (at.row + m0) * a.ldy + col, r0 = (at.row + m0) * a.ldr + col;
 #pragma unroll
     for (int j0 = 0; j0 < C::FJ; j0 += G) {
@@ -166,25 +167,28 @@ __device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& 
   }
 }
 
-// The same where columns of the tile lie past N: 16 rows at a time through `lds` (64 bytes a column), element by
-// element in the columns' order.
+// The last N % 8 columns, which no lane of finish_as has: 16 rows at a time through `lds` (512 bytes a wave), element
+// by element in the columns' order.
 template <class C>
-__device__ __forceinline__ void finish_ragged(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
-                                              int col0, int lane, int mine, int of, float* lds) {
+__device__ __forceinline__ void finish_last(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ], int wm,
+                                            int col0, int lane, int mine, int of, float* lds) {
+  const int last = a.N & ~7;
 #pragma unroll
-  for (int j = 0; j < C::FJ; ++j) {
+  for (int p = 0; p < C::FI / 2; ++p) {
+    const int piece = col0 + p * 32;
+    if (last < piece || last >= piece + 32) continue;
 #pragma unroll
-    for (int p = 0; p < C::FI / 2; ++p) {
+    for (int j = 0; j < C::FJ; ++j) {
       if ((p * C::FJ + j) % of != mine) continue;
-      const int c = p * 32 + (lane >> 4) * 8;
+      if (piece + (lane >> 4) * 8 == last) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) lds[(lane & 15) * C::TN + c + q] = acc[2 * p + q / 4][j][q % 4];
+        for (int q = 0; q < 8; ++q) lds[(lane & 15) * 8 + q] = acc[2 * p + q / 4][j][q % 4];
+      }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      for (int i = lane; i < 16 * 32; i += 64) {
-        const int m = wm + j * 16 + i / 32, col = col0 + p * 32 + i % 32;
-        if (m < at.rows && col < a.N)
-          finish1<typename C::T>(a, at.e, (int64_t)at.row + m, col, lds[i / 32 * C::TN + p * 32 + i % 32]);
+      for (int i = lane; i < 128; i += 64) {
+        const int m = wm + j * 16 + i / 8, col = last + i % 8;
+        if (m < at.rows && col < a.N) finish1<typename C::T>(a, at.e, (int64_t)at.row + m, col, lds[i]);
       }
       __builtin_amdgcn_wave_barrier();
     }
@@ -195,15 +199,12 @@ template <class C>
 __device__ __forceinline__ void finish(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ],
                                        const Bias<C>& bias, int wm, int n0, int wn, int lane, int mine, int of, char* lds,
                                        int wave) {
-  if (n0 + C::BN > a.N) {
+  if (a.act <= DML_ACT_RELU) finish_as<kClamp, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+  else if (a.act == DML_ACT_GELU) finish_as<kErf, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+  else finish_as<kSwish, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+  if ((a.N & 7) && n0 + C::BN > a.N) {
     __syncthreads();
-    finish_ragged<C>(a, at, acc, wm, n0 + wn, lane, mine, of, (float*)lds + wave * 16 * C::TN);
-  } else if (a.act <= DML_ACT_RELU) {
-    finish_as<kClamp, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
-  } else if (a.act == DML_ACT_GELU) {
-    finish_as<kErf, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
-  } else {
-    finish_as<kSwish, C>(a, at, acc, bias, wm, n0 + wn, lane, mine, of);
+    finish_last<C>(a, at, acc, wm, n0 + wn, lane, mine, of, (float*)lds + wave * 128);
   }
 }
 
