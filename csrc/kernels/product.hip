@@ -574,30 +574,34 @@ static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
   return 0;
 }
 
-// The tiled forms a product can run in, and what each costs in microseconds behind the launch: `fixed` a tile (its
-// ends), and a slice of 64 (KG of them) `alone` where a CU has one such workgroup at a time, `shared` times their
-// number where it has more (the L2's rate, or the matrix cores' for the largest). Measured over 1 to 16384 rows, K 256
-// to 8192, N 256 to 8192 (256 x 4096 x 4096: 32.2 / 24.1 / 20.1 us with KG 1 / 2 / 4; 1024 x 512 x 2048: 7.6 / 8.6 /
-// 11.3; 17664 x 1024 x 4096: 192 us in tiles of 256, 160 of 192 x 128, 180 of 128; 16384 x 4096 x 4096: 430 / 462 /
-// 500; 6304 x 4096 x 1024: 83 / 76 / 54).
+// The tiled forms a product can run in, and what each costs in microseconds: `first` once, `fixed` a tile (its ends),
+// and a slice of 64 (KG of them) from `low`, on a card that is otherwise idle, to `high`, with a workgroup on every CU,
+// for as many workgroups as a CU holds, or `shared` times their number if that is more. Fitted to 2000 timings over 1 to
+// 12000 rows, K 64 to 8192, N 32 to 7000; of those 260 products the form chosen is 1.4 % slower than the best of all in
+// the mean, 19 % at worst. Where each wins: 300 x 6144 x 346 takes 14.7 us in tiles of 32 with KG = 8 and 25.9 in tiles of
+// 64 with 4 (more workgroups to load); 1024 x 512 x 2048 7.6 with KG = 1, 8.6 with 2, 11.3 with 4; 17664 x 1024 x 4096 192
+// in tiles of 256, 160 of 192 x 128, 180 of 128; 16384 x 4096 x 4096 430 / 462 / 500; 6304 x 4096 x 1024 83 / 76 / 54.
 struct Form {
   int bm, bn, kg, per_cu;
-  double fixed, alone, shared;
+  double first, fixed, low, high, shared;
 };
-constexpr Form kForms[] = {{64, 64, 1, 4, 1.0, 0.47, 0.25}, {64, 64, 2, 2, 1.0, 0.62, 0.5}, {64, 64, 4, 1, 1.5, 1.05, 1.05},
-                           {128, 128, 1, 2, 3.0, 0.65, 0.46}, {192, 128, 1, 2, 3.5, 0.81, 0.6}, {256, 256, 1, 1, 12.0, 1.6, 1.6}};
+constexpr Form kForms[] = {{32, 32, 8, 1, 1.8, 2.3, 0.50, 0.84, 0},     {64, 64, 1, 4, 2.7, 0.6, 0.21, 0.44, 0.18},
+                           {64, 64, 2, 2, 2.3, 1.4, 0.30, 0.69, 0},     {64, 64, 4, 1, 1.9, 2.7, 0.51, 0.99, 0},
+                           {128, 128, 1, 2, 2.5, 2.6, 0.41, 0.81, 0.42}, {192, 128, 1, 2, 2.8, 3.6, 0.57, 1.09, 0},
+                           {256, 256, 1, 1, 0, 7.9, 1.09, 1.61, 0}};
 
 static long tiles_of(const DmlProductArgs* a, int bm, int bn) { return row_tiles(a, bm) * ((a->N + bn - 1) / bn); }
 
 static double cost(const DmlProductArgs* a, const Form& f, bool dma) {
-  const long per = (tiles_of(a, f.bm, f.bn) + 255) / 256, rounds = per / f.per_cu, rest = per % f.per_cu;
-  const auto slice = [&](long n) { return n == 0 ? 0.0 : n * f.shared > f.alone ? n * f.shared : f.alone; };
+  const long tiles = tiles_of(a, f.bm, f.bn), per = (tiles + 255) / 256, rounds = per / f.per_cu, rest = per % f.per_cu;
+  const double one = f.low + (f.high - f.low) * (tiles < 256 ? tiles / 256.0 : 1.0);
+  const auto slice = [&](long n) { return n == 0 ? 0.0 : n * f.shared > one ? n * f.shared : one; };
   // rows off the 128-byte lines: a slice takes two lines each, which costs the forms that the L2 bounds (5000 x 2000 x
   // 6000 bf16: 134 us in tiles of 256, 153 of 192 x 128)
   const double lines = f.bm < 256 && ((a->ldx | a->ldw) & 63) ? 1.2 : 1.0;
   const int slices = (a->K + 64 * f.kg - 1) / (64 * f.kg);
   const double t = lines * slices * (rounds * slice(f.per_cu) + slice(rest)) + per * f.fixed;
-  return dma ? t : 1.4 * t + (f.kg > 1 ? 2.5 : 0);  // through registers
+  return f.first + (dma ? t : 1.4 * t + (f.kg > 1 ? 4 : 2));  // through registers
 }
 
 template <class T>
@@ -606,26 +610,29 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   const bool dma = a->K % 8 == 0 && a->ldx % 8 == 0 && a->ldw % 8 == 0 && a->w_group % 8 == 0 &&
                    (((uintptr_t)a->x | (uintptr_t)a->w) & 15) == 0 && a->ldx < (1 << 22) && a->ldw < (1 << 22) &&
                    255 * (a->ldx > a->ldw ? a->ldx : a->ldw) + a->K < (1 << 30) - 512 && a->K < (1 << 22);
-  // product_rows in 16 x 16 (16 waves: 2048 of K in flight) and 32 x 32 (8 waves, 512): a workgroup on a CU takes 3.5 us
-  // per 2048 of K and 1.9 per 512 (17 x 3000 x 1000: 8.6 us, 500 x 500 x 500: 5.8, the best tile 12 and 8)
-  const double k = a->K / 2048.0;
-  const double rows16 = (tiles_of(a, 16, 16) + 255) / 256 * (k < 0.45 ? 0.45 : k) * 3.5 + 0.5;
-  const double rows32 = (tiles_of(a, 32, 32) + 255) / 256 * ((a->K + 511) / 512) * 1.9 + 1.0;
+  // product_rows in 16 x 16 (16 waves: 2048 of K in flight) and 32 x 32 (8 waves, 512), by the same timings: a workgroup
+  // on a CU takes 3.6 us per 2048 of K, less where there is one tile of rows, and 1.3 to 1.6 per 512 (more
+  // off the dword grid: 67 x 519 x 1388 takes 6.8 us in 16 x 16, 7.9 in 32 x 32)
+  const double k = a->K / 2048.0, t32 = (double)tiles_of(a, 32, 32);
+  const double rows16 = 3.1 + (tiles_of(a, 16, 16) + 255) / 256 * (k < 0.45 ? 0.45 : k) * (a->M <= 16 ? 3.0 : 3.6);
+  const double each32 = 1.3 + 0.3 * (t32 < 256 ? t32 / 256 : 1.0), all32 = ((long)t32 + 255) / 256 * ((a->K + 511) / 512) * each32;
+  const double rows32 = dma ? 3.1 + all32 : 3.8 + 1.25 * all32;
   double least = rows16 < rows32 ? rows16 : rows32;
   int best = rows16 < rows32 ? -1 : -2;
   for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
-    if (!dma && (kForms[i].bm > 128 || kForms[i].kg == 2)) continue;  // not built through registers
+    if (!dma && (kForms[i].bm > 128 || kForms[i].kg == 2 || kForms[i].kg == 8)) continue;  // not built through registers
     const double c = cost(a, kForms[i], dma);
     if (c < least) least = c, best = i;
   }
   switch (best) {
     case -2: return launch_rows<T, 2, 8, 1>(a, s);
     case -1: return launch_rows<T, 1, 16, 2>(a, s);
-    case 0: return dma ? launch<Tile<T, 64, 64, 2, 2, 1, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 1, false>>(a, s);
-    case 1: return launch<Tile<T, 64, 64, 2, 2, 2, true>>(a, s);
-    case 2: return dma ? launch<Tile<T, 64, 64, 2, 2, 4, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 4, false>>(a, s);
-    case 3: return dma ? launch<Tile<T, 128, 128, 2, 2, 1, true>>(a, s) : launch<Tile<T, 128, 128, 2, 2, 1, false>>(a, s);
-    case 4: return launch<Tile<T, 192, 128, 2, 2, 1, true>>(a, s);
+    case 0: return launch<Tile<T, 32, 32, 1, 1, 8, true>>(a, s);
+    case 1: return dma ? launch<Tile<T, 64, 64, 2, 2, 1, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 1, false>>(a, s);
+    case 2: return launch<Tile<T, 64, 64, 2, 2, 2, true>>(a, s);
+    case 3: return dma ? launch<Tile<T, 64, 64, 2, 2, 4, true>>(a, s) : launch<Tile<T, 64, 64, 2, 2, 4, false>>(a, s);
+    case 4: return dma ? launch<Tile<T, 128, 128, 2, 2, 1, true>>(a, s) : launch<Tile<T, 128, 128, 2, 2, 1, false>>(a, s);
+    case 5: return launch<Tile<T, 192, 128, 2, 2, 1, true>>(a, s);
     default: return launch<Tile<T, 256, 256, 2, 4, 1, true>>(a, s);
   }
 }

@@ -254,7 +254,9 @@ def operands(g, m, k, n, dtype):
 SIZES = [(1, 1, 1), (1, 16, 1000), (1, 2048, 1000), (1, 4099, 33), (2, 64, 64), (3, 100, 17), (16, 512, 256),
          (17, 520, 264), (31, 1024, 48), (64, 64, 64), (65, 33, 129), (100, 2048, 100), (128, 4096, 512),
          (200, 72, 4096), (256, 256, 256), (257, 1000, 257), (333, 1001, 517), (512, 128, 1024), (1000, 768, 776),
-         (1, 8192, 8192), (5, 8191, 1023), (2000, 8, 40), (700, 2056, 520), (2049, 192, 264), (4100, 64, 8)]
+         (1, 8192, 8192), (5, 8191, 1023), (2000, 8, 40), (700, 2056, 520), (2049, 192, 264), (4100, 64, 8),
+         (300, 6144, 346), (33, 2048, 70), (40, 1032, 530), (1030, 2048, 2052), (4020, 960, 3508), (8200, 520, 4100),
+         (1500, 4096, 1001), (150, 4728, 1730), (2500, 1001, 3000), (600, 2047, 600)]
 
 
 @pytest.mark.parametrize("dtype", (BF, HF))
