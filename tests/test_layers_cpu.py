@@ -116,6 +116,26 @@ def test_argument_structs_match_the_library():
     N.lib()
 
 
+def test_older_library_is_checked_for_the_structs_it_has(monkeypatch):
+    """A library from before the last struct loads only where it is asked for by path; a size that differs never does."""
+    def library(known, off=0):
+        def sizes(out, n):
+            for i, name in enumerate(N.ABI_STRUCTS[:known]):
+                out[i] = C.sizeof(getattr(N, name)) + off
+            return known
+        return type("Library", (), {"dml_abi_sizes": staticmethod(sizes)})
+
+    count = len(N.ABI_STRUCTS)
+    monkeypatch.delenv("DML_LIB", raising=False)
+    N._check_abi(library(count))
+    with pytest.raises(N.NativeError):
+        N._check_abi(library(count - 1))
+    monkeypatch.setenv("DML_LIB", "older.so")
+    N._check_abi(library(count - 1))
+    with pytest.raises(N.NativeError):
+        N._check_abi(library(count - 1, off=8))
+
+
 def _norm_args(**kw):
     d = {"x": 16, "y": 16, "weight": 0, "bias": 0, "xn": 64, "yn": 64, "ldx": 16, "ldy": 16, "ws": 0, "ws_bytes": 0,
          "N": 1, "HW": 4, "C": 16, "G": 4, "dtype": 0, "act": 0, "eps": 1e-5, **kw}
