@@ -571,6 +571,17 @@ def test_grouped_linear_shared_weight_and_many_groups():
     check_grouped(g, [0, 1, 2, 0, 0, 3] * 170, 32, 48, BF, "relu", spare=5)
 
 
+@pytest.mark.parametrize("e", (63, 64, 65, 300, 4095, 4096, 4097, 9000))
+@pytest.mark.parametrize("ascending", (True, False))
+def test_grouped_linear_finds_its_groups(e, ascending):
+    """Few rows over many groups, most of them empty; ends out of order are clamped as in any call."""
+    g = torch.Generator().manual_seed(e)
+    ends = torch.randint(-3, 150, (e,), generator=g)
+    if ascending:
+        ends = ends.sort().values
+    check_grouped(gen(e), [0] * (e - 1) + [140], 16, 24, BF, spare=20, ends=ends.tolist())
+
+
 @pytest.mark.parametrize("m, k, n", [(70000, 8, 16), (40000, 136, 24), (3, 40000, 64), (20, 16, 30000), (66000, 64, 1)])
 def test_linear_long_and_thin(m, k, n):
     g = gen(73)
