@@ -577,7 +577,7 @@ static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
 // The tiled forms a product can run in, and what each costs in microseconds: `first` once, `fixed` a tile (its ends),
 // and a slice of 64 (KG of them) from `low`, on a card that is otherwise idle, to `high`, with a workgroup on every CU,
 // for as many workgroups as a CU holds, or `shared` times their number if that is more. Fitted to 2000 timings over 1 to
-// 12000 rows, K 64 to 8192, N 32 to 7000; of those 260 products the form chosen is 1.4 % slower than the best of all in
+// 12000 rows, K 64 to 8192, N 32 to 7000; of 255 of those products the form chosen is 1.4 % slower than the best of all in
 // the mean, 19 % at worst. Where each wins: 300 x 6144 x 346 takes 14.7 us in tiles of 32 with KG = 8 and 25.9 in tiles of
 // 64 with 4 (more workgroups to load); 1024 x 512 x 2048 7.6 with KG = 1, 8.6 with 2, 11.3 with 4; 17664 x 1024 x 4096 192
 // in tiles of 256, 160 of 192 x 128, 180 of 128; 16384 x 4096 x 4096 430 / 462 / 500; 6304 x 4096 x 1024 83 / 76 / 54.
