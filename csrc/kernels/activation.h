@@ -36,8 +36,9 @@ __device__ __forceinline__ float swish(float v, float a, float b) {
 
 // The activations (DML_ACT_*) as three kinds of code, each with two parameters:
 //   none, relu       max(v, a), a = -infinity or 0 (by comparison: NaN stays NaN)
-//   silu, gelu_tanh  v / (1 + 2^-(a v + b v^3)): a = 1 / ln 2, b = 0 for silu; gelu_tanh(v) = v/2 (1 + tanh u)
-//                    = v / (1 + e^-2u), u = sqrt(2/pi) (v + 0.044715 v^3)
+//   silu, gelu_tanh  v / (1 + 2^-(a v + b v^3)): a = 1 / ln 2, b the least normal number for silu (0 times infinity
+//                    would be NaN; b v^2 is below a's rounding up to |v| = 10^15, where 2^-av is long 0 or infinite);
+//                    gelu_tanh(v) = v/2 (1 + tanh u) = v / (1 + e^-2u), u = sqrt(2/pi) (v + 0.044715 v^3)
 //   gelu             v Phi(v)
 // exp and 1/x are the hardware's, good to a step or two: 1e-7 relative each.
 enum { kClamp, kSwish, kErf };
@@ -50,7 +51,7 @@ struct Act {
 };
 __device__ __forceinline__ Act act_parameters(int act) {
   return act <= DML_ACT_RELU ? Act{act == DML_ACT_RELU ? 0.f : -INFINITY, 0.f}
-         : act == DML_ACT_GELU_TANH ? Act{2.3022081981f, 0.102943239580f} : Act{1.4426950409f, 0.f};
+         : act == DML_ACT_GELU_TANH ? Act{2.3022081981f, 0.102943239580f} : Act{1.4426950409f, 0x1p-126f};
 }
 // one value, of a wave-uniform `act`
 __device__ __forceinline__ float activate(float v, int act) {
