@@ -319,14 +319,16 @@ __global__ __launch_bounds__(NT) void stats(DmlGroupNormArgs a, int S, int rows,
 // All rows' (mean, M2) of a group from its `parts` of `rows` rows each, by L lanes of a wave: every lane has it.
 template <int L>
 __device__ __forceinline__ float2 joined(const float2* ws, int parts, int rows, int HW, int cg, int lane) {
+  // a part may hold 2^31 values and more
+  const auto weight = [&](int i) { return (float)min(rows, HW - i * rows) * (float)cg; };
   float sum = 0.f, m2 = 0.f;
 #pragma unroll 4
-  for (int i = lane; i < parts; i += L) sum += ws[i].x * (float)(min(rows, HW - i * rows) * cg);
+  for (int i = lane; i < parts; i += L) sum += ws[i].x * weight(i);
   const float mu = over_lanes<L>(sum) / ((float)HW * (float)cg);
 #pragma unroll 4
   for (int i = lane; i < parts; i += L) {
     const float d = ws[i].x - mu;
-    m2 += ws[i].y + d * d * (float)(min(rows, HW - i * rows) * cg);
+    m2 += ws[i].y + d * d * weight(i);
   }
   return make_float2(mu, over_lanes<L>(m2));
 }

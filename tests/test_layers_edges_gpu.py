@@ -50,3 +50,18 @@ def test_group_norm_at_infinity(shape, groups, act, dtype):
     b[1], b[2] = INF, -INF
     want[..., 1:3] = act64(b[1:3].double(), act).to(dtype)
     assert same(ops.group_norm(x, groups, None, b, act=act), want)
+
+
+# ---------------------------------------------------------------- group norm
+
+
+@pytest.mark.parametrize("positions, c", [(2 ** 23, 256), (2 ** 26, 64), (2 ** 25 + 4097, 80), (2 ** 29, 64)])
+def test_group_norm_of_groups_beyond_31_bits(positions, c):
+    """One group of 2^31 to 2^35 values, half of them 1 and half 3: mean 2, variance 1, so -1 and 1 in bf16 (0.999995
+    rounds to it, and stays there for errors of the statistics up to 2^-10)."""
+    row = torch.tensor([1.0, 3.0], device="cuda", dtype=BF).repeat(c // 2)
+    y = ops.group_norm(row.expand(1, positions, c), 1)
+    for part in y[0].split(2 ** 22):
+        assert (part == row - 2).all()
+    del y, part
+    torch.cuda.empty_cache()
