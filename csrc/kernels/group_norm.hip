@@ -169,10 +169,10 @@ __device__ __forceinline__ void read_and_sum(const Slab<T, NT, CH>& s, const T* 
       float n0 = 0.f, s0 = 0.f, s1 = 0.f, q0 = 0.f, q1 = 0.f;
 #pragma unroll
       for (int p = 0; p < V; ++p) {
-        const float w0 = p >= s.lo && p < cut ? 1.f : 0.f, w1 = p >= cut ? 1.f : 0.f;
-        n0 += w0;
-        s0 += w0 * mean[p];
-        s1 += w1 * mean[p];
+        const bool in0 = p >= s.lo && p < cut, in1 = p >= cut;  // selected: a product with 0 would pass NaN on
+        n0 += in0 ? 1.f : 0.f;
+        s0 += in0 ? mean[p] : 0.f;
+        s1 += in1 ? mean[p] : 0.f;
       }
       const float mu0 = s0 / n0, mu1 = cut < V ? s1 / (float)(V - cut) : 0.f;
 #pragma unroll

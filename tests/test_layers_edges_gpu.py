@@ -55,6 +55,29 @@ def test_group_norm_at_infinity(shape, groups, act, dtype):
 # ---------------------------------------------------------------- group norm
 
 
+@pytest.mark.parametrize("dtype", (BF, FP))
+@pytest.mark.parametrize("shape, groups", [((2, 50, 72), 8), ((2, 35, 35, 288), 32), ((2, 20, 100), 10), ((3, 20, 55), 5),
+                                           ((2, 40, 40), 8), ((2, 30, 39), 3), ((2, 9000, 99), 9), ((1, 9000, 130), 10),
+                                           ((2, 20, 14), 2), ((2, 20, 21), 7)])
+@pytest.mark.parametrize("bad", (NAN, INF, -INF))
+def test_group_norm_keeps_bad_values_to_groups_that_cut_vectors(shape, groups, bad, dtype):
+    """Groups whose width is no multiple of a vector's: each in turn, at its first and last channel."""
+    g = gen(13)
+    clean = normal(g, *shape).to(dtype)
+    want = ops.group_norm(clean, groups, act="gelu")
+    assert not want.isnan().any()
+    cg = shape[-1] // groups
+    n = shape[0] - 1
+    for k in range(groups):
+        for c in (k * cg, (k + 1) * cg - 1):
+            x = clean.clone()
+            x[n].reshape(-1, shape[-1])[7, c] = bad
+            y = ops.group_norm(x, groups, act="gelu")
+            hit = torch.zeros(shape, dtype=torch.bool, device="cuda")
+            hit[n, ..., k * cg:(k + 1) * cg] = True
+            assert y[hit].isnan().all() and torch.equal(y[~hit], want[~hit]), (k, c)
+
+
 @pytest.mark.parametrize("positions, c", [(2 ** 23, 256), (2 ** 26, 64), (2 ** 25 + 4097, 80), (2 ** 29, 64)])
 def test_group_norm_of_groups_beyond_31_bits(positions, c):
     """One group of 2^31 to 2^35 values, half of them 1 and half 3: mean 2, variance 1, so -1 and 1 in bf16 (0.999995
