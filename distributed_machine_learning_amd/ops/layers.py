@@ -63,8 +63,9 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return p, p + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def _apart(out: torch.Tensor, same: Optional[torch.Tensor], **others: Optional[torch.Tensor]) -> None:
-    """out must share no memory with the others unless they are other columns of one buffer; it may be `same` itself."""
+def _apart(out: torch.Tensor, same: str, **others: Optional[torch.Tensor]) -> None:
+    """out must share no memory with the others unless they are other columns of one buffer. It may be the one named
+    `same` itself (each workgroup reads its part before it writes there), but not where that is passed as another one too."""
     if not out.numel():
         return
     a, b = _span(out)
@@ -74,7 +75,7 @@ def _apart(out: torch.Tensor, same: Optional[torch.Tensor], **others: Optional[t
         c, d = _span(t)
         if b <= c or d <= a:
             continue
-        if t is same and a == c and out.shape == t.shape and out.stride() == t.stride() and out.dtype == t.dtype:
+        if what == same and a == c and out.shape == t.shape and out.stride() == t.stride() and out.dtype == t.dtype:
             continue
         steps = [s for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1]
         if steps and out.element_size() == t.element_size() and out.stride() == t.stride() \
@@ -161,7 +162,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         _, ldy = _pitch(out, 1, "out")
         if (rows > 1 and ldy < c) or (n > 1 and out.stride(0) < c):
             raise ValueError("out: its positions overlap each other")
-        _apart(out, x, x=x, weight=weight, bias=bias)
+        _apart(out, "x", x=x, weight=weight, bias=bias)
     if max(n, rows, c, n * groups) > _INT - 4096:
         raise ValueError("x: over 2^31 - 4097 samples, positions, channels or groups")
     device = _ready(x, weight, bias, out)
@@ -217,7 +218,7 @@ def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, wha
         ldy = _pitch(out, 0, "out")[1]
         if m > 1 and ldy < n:
             raise ValueError("out: its rows overlap each other")
-        _apart(out, residual, x=x, weight=weight, bias=bias, ends=ends, residual=residual)
+        _apart(out, "residual", x=x, weight=weight, bias=bias, ends=ends, residual=residual)
     if max(m, n, e) > _INT - 512 or k > 2 ** 30:
         raise ValueError(f"{what}: a dimension over 2^31 - 513, or K over 2^30")
     device = _ready(x, weight, ends, bias, residual, out)

@@ -180,3 +180,17 @@ def test_library_product_of_nothing():
     assert N.lib().dml_product(_prod_args(M=0), None) == 0
     assert N.lib().dml_product(_prod_args(N=0), None) == 0
     assert N.lib().dml_product(None, None) == -1
+
+
+@pytest.mark.parametrize("what, call", [
+    ("x", lambda t: ops.linear(t, _t(8, 8), residual=t, out=t)),
+    ("x", lambda t: ops.linear(t, _t(8, 8), residual=t, act_last=True, act="relu", out=t)),
+    ("weight", lambda t: ops.linear(_t(8, 8), t, residual=t, out=t)),
+    ("x", lambda t: ops.grouped_linear(t, _t(2, 8, 8), torch.tensor([1, 8]), residual=t, out=t)),
+    ("bias", lambda t: ops.grouped_linear(_t(8, 8), _t(8, 8, 8), torch.arange(8), bias=t, residual=t, out=t)),
+    ("weight", lambda t: ops.group_norm(t[0].view(1, 1, 8), 4, weight=t[0], out=t[0].view(1, 1, 8))),
+])
+def test_out_that_is_the_residual_and_another_operand_too(what, call):
+    """One tensor in two places: x and weight are read by many workgroups, so out is refused, object or view alike."""
+    with pytest.raises(ValueError, match=f"out overlaps {what}"):
+        call(_t(8, 8))
