@@ -160,7 +160,9 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
         if out.shape != x.shape or out.dtype is not x.dtype:
             raise ValueError(f"out: expected {x.dtype} of shape {tuple(x.shape)}, got {out.dtype} of {tuple(out.shape)}")
         _, ldy = _pitch(out, 1, "out")
-        if (rows > 1 and ldy < c) or (n > 1 and out.stride(0) < c):
+        # positions apart, and samples behind each other ([N, L, C]) or between the positions of one ([L, N, C] seen so)
+        step = out.stride(0) if n > 1 else _INT
+        if rows > 1 and ldy < c or step < c or step < (rows - 1) * ldy + c and ldy < (n - 1) * step + c:
             raise ValueError("out: its positions overlap each other")
         _apart(out, "x", x=x, weight=weight, bias=bias)
     if max(n, rows, c, n * groups) > _INT - 4096:

@@ -194,3 +194,22 @@ def test_out_that_is_the_residual_and_another_operand_too(what, call):
     """One tensor in two places: x and weight are read by many workgroups, so out is refused, object or view alike."""
     with pytest.raises(ValueError, match=f"out overlaps {what}"):
         call(_t(8, 8))
+
+
+@pytest.mark.parametrize("shape, strides, fits", [
+    ((4, 9, 16), (16, 16, 1), False),    # windows over one sequence: samples share eight of nine positions
+    ((2, 9, 16), (143, 16, 1), False),   # by one element
+    ((2, 9, 16), (144, 16, 1), True),
+    ((2, 9, 16), (16, 32, 1), True),     # samples between the positions of the first
+    ((3, 9, 16), (16, 32, 1), False),
+    ((3, 9, 16), (20, 56, 1), True),
+    ((3, 9, 16), (20, 55, 1), False),
+    ((2, 1, 16), (16, 1, 1), True),
+    ((2, 1, 16), (15, 1, 1), False),
+    ((2, 2, 3, 16), (40, 48, 16, 1), False),
+    ((1, 9, 16), (1, 16, 1), True),
+])
+def test_group_norm_out_that_overlaps_itself(shape, strides, fits):
+    out = torch.zeros(2000, dtype=BF).as_strided(shape, strides)
+    with pytest.raises(ValueError, match="HIP device" if fits else "overlap each other"):
+        ops.group_norm(_t(*shape), 4, out=out)
