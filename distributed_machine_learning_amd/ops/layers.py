@@ -77,13 +77,15 @@ def _apart(out: torch.Tensor, same: str, **others: Optional[torch.Tensor]) -> No
             continue
         if what == same and a == c and out.shape == t.shape and out.stride() == t.stride() and out.dtype == t.dtype:
             continue
-        steps = [s for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1]
-        if steps and out.element_size() == t.element_size() and out.stride() == t.stride() \
-                and out.shape[:-1] == t.shape[:-1]:
-            pitch = min(steps) * out.element_size()
-            gap = (c - a) % pitch  # t's columns begin here in out's rows
-            if abs(c - a) < pitch and gap >= out.shape[-1] * out.element_size() \
-                    and gap + t.shape[-1] * t.element_size() <= pitch:
+        size = out.element_size()
+        if size == t.element_size() and out.stride() == t.stride() and out.shape[:-1] == t.shape[:-1]:
+            a1, c1 = a + out.shape[-1] * size, c + t.shape[-1] * size  # behind the first rows
+            span = max(a1, c1) - min(a, c)
+            fits = a1 <= c or c1 <= a
+            for step, n in sorted((s * size, n) for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1):
+                fits = fits and step >= span  # what both cover so far repeats without meeting itself
+                span += (n - 1) * step
+            if fits:
                 continue
         raise ValueError(f"out overlaps {what}")
 

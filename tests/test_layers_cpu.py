@@ -213,3 +213,22 @@ def test_group_norm_out_that_overlaps_itself(shape, strides, fits):
     out = torch.zeros(2000, dtype=BF).as_strided(shape, strides)
     with pytest.raises(ValueError, match="HIP device" if fits else "overlap each other"):
         ops.group_norm(_t(*shape), 4, out=out)
+
+
+@pytest.mark.parametrize("steps, other, fits", [
+    ((96, 32), 16, True), ((128, 32), 16, True), ((112, 32), 16, True),
+    ((80, 32), 16, False),                       # the second sample of x begins where out's third position lies
+    ((95, 32), 16, False),
+    ((110, 40), 24, False), ((110, 40), 16, False), ((112, 40), 16, True), ((120, 40), 24, True), ((120, 40), 25, False),
+    ((120, 40), 15, False), ((120, 40), -16, True), ((120, 40), -24, True), ((120, 40), -25, False), ((120, 40), 40, False),
+    ((32, 64), 16, True), ((31, 64), 16, False), ((32, 63), 16, False),  # samples between the positions of the first
+])
+def test_group_norm_out_in_other_columns(steps, other, fits):
+    """Other columns of the same rows, by x's strides."""
+    buf = torch.zeros(500, dtype=BF)
+    shape = (2, 3, 16)
+    x, out = (buf.as_strided(shape, (*steps, 1), at) for at in (40, 40 + other))
+    mine, theirs = (set((torch.arange(500).as_strided(shape, (*steps, 1), at)).flatten().tolist()) for at in (40, 40 + other))
+    assert fits == (not mine & theirs)
+    with pytest.raises(ValueError, match="HIP device" if fits else "out overlaps x"):
+        ops.group_norm(x, 4, out=out)
