@@ -13,6 +13,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as N
 
@@ -98,7 +99,7 @@ def _vector(v: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, what: s
 
 
 def _ready(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
-    """x's device number: all are on one HIP device, and none is one that autograd would expect a gradient for."""
+    """x's device number: all are on one HIP device, and none is one that autograd would expect a derivative for."""
     dev = x.get_device()
     grad = torch.is_grad_enabled()
     if grad and x.requires_grad:
@@ -109,6 +110,10 @@ def _ready(x: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
                 raise ValueError(f"tensors on different devices: {x.device} and {t.device}")
             if grad and t.requires_grad:
                 raise ValueError("this operator has no backward: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:  # inside a dual_level; no_grad does not stop tangents
+        for t in (x, *others):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("this operator has no derivative: call it on unpack_dual(t).primal")
     if dev < 0:
         raise ValueError(f"expected tensors on a HIP device, got {x.device}")
     return dev

@@ -3,6 +3,7 @@ import ctypes as C
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from distributed_machine_learning_amd import _native as N
 from distributed_machine_learning_amd import ops
@@ -232,3 +233,23 @@ def test_group_norm_out_in_other_columns(steps, other, fits):
     assert fits == (not mine & theirs)
     with pytest.raises(ValueError, match="HIP device" if fits else "out overlaps x"):
         ops.group_norm(x, 4, out=out)
+
+
+@pytest.mark.parametrize("no_grad", (False, True))
+@pytest.mark.parametrize("call", [
+    lambda d: _norm(d(_t(2, 3, 3, 16))), lambda d: _norm(weight=d(_t(16))), lambda d: _norm(bias=d(_t(16))),
+    lambda d: _norm(out=d(_t(2, 3, 3, 16))), lambda d: _lin(d(_t(4, 8))), lambda d: _lin(w=d(_t(6, 8))),
+    lambda d: _lin(bias=d(_t(6))), lambda d: _lin(residual=d(_t(4, 6))), lambda d: _grp(d(_t(4, 8))), lambda d: _grp(w=d(_t(2, 6, 8))),
+])
+def test_forward_mode_tangents_are_refused(call, no_grad):
+    """Results without the tangent would be wrong derivatives, with no error; tensors without one pass in a dual level."""
+    with torch.set_grad_enabled(not no_grad), forward_ad.dual_level():
+        with pytest.raises(ValueError, match="no derivative"):
+            call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+        with pytest.raises(ValueError, match="HIP device"):
+            call(lambda t: t)
+
+
+def test_forward_mode_through_a_function_transform():
+    with pytest.raises(ValueError, match="no derivative"):
+        torch.func.jvp(lambda t: _norm(t), (_t(2, 3, 3, 16),), (_t(2, 3, 3, 16),))
