@@ -111,7 +111,7 @@ struct Bias {
 
 // A wave's accumulators (rows wm.., columns col0..) through the epilogue: of its 16 x 32 pieces those whose number is
 // `mine` modulo `of`. A lane has eight columns of a row in a piece, and leaves them out unless all are inside. The
-// residuals of G pieces are read ahead of the stores, which could be to the same memory.
+// residuals of its pieces are read G at a time ahead of the stores, which could be to the same memory.
 template <int KIND, class C>
 __device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& at, f32x4 (&acc)[C::FI][C::FJ],
                                           const Bias<C>& bias, int wm, int col0, int lane, int mine, int of) {
@@ -130,7 +130,7 @@ __device__ __forceinline__ void finish_as(const DmlProductArgs& a, const Place& 
       if (a.res) {
 #pragma unroll
         for (int j = 0; j < G; ++j)
-          if (m0 + (j0 + j) * 16 < at.rows) {
+          if ((p * C::FJ + j0 + j) % of == mine && m0 + (j0 + j) * 16 < at.rows) {
             const int64_t i = r0 + (j0 + j) * 16 * a.ldr;
             if (a.out_f32) {
               __builtin_memcpy(r[j], (const float*)a.res + i, 32);

@@ -88,3 +88,24 @@ def test_group_norm_of_groups_beyond_31_bits(positions, c):
         assert (part == row - 2).all()
     del y, part
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------- products
+
+
+@pytest.mark.parametrize("out_dtype", (BF, FP))
+@pytest.mark.parametrize("m, k, n", [(300, 6144, 346), (64, 8192, 1024), (150, 4728, 1730), (256, 4096, 4096), (563, 4584, 2515),
+                                     (1024, 512, 2048), (200, 2001, 600), (9, 4096, 264)])
+def test_products_into_their_residual(m, k, n, out_dtype):
+    """Sums that several sets of waves hold, each finishing its own part: the residual is read where they then write."""
+    g = gen(m + n)
+    x, w, b = normal(g, m, k).to(BF), (normal(g, n, k) * k ** -0.5).to(BF), normal(g, n)
+    ends, pair = torch.tensor([m // 3, m], device="cuda"), torch.stack([w, -w])
+    r = normal(g, m, n).to(out_dtype)
+    kw = {"act": "gelu", "out_dtype": out_dtype}
+    want = ops.linear(x, w, b, residual=r, **kw), ops.grouped_linear(x, pair, ends, residual=r, act_last=True, **kw)
+    for _ in range(3):
+        y, z = r.clone(), r.clone()
+        ops.linear(x, w, b, residual=y, out=y, **kw)
+        ops.grouped_linear(x, pair, ends, residual=z, act_last=True, out=z, **kw)
+        assert torch.equal(y, want[0]) and torch.equal(z, want[1])
