@@ -586,7 +586,7 @@ struct Form {
   double first, fixed, low, high, shared;
 };
 constexpr Form kForms[] = {{32, 32, 8, 1, 1.8, 2.3, 0.50, 0.84, 0},     {64, 64, 1, 4, 2.7, 0.6, 0.21, 0.44, 0.18},
-                           {64, 64, 2, 2, 2.8, 1.4, 0.30, 0.69, 0},     {64, 64, 4, 1, 1.9, 2.7, 0.51, 0.99, 0},
+                           {64, 64, 2, 2, 2.3, 1.4, 0.30, 0.69, 0},     {64, 64, 4, 1, 1.9, 2.7, 0.51, 0.99, 0},
                            {128, 128, 1, 2, 2.5, 2.6, 0.41, 0.81, 0.42}, {192, 128, 1, 2, 2.8, 3.6, 0.57, 1.09, 0},
                            {256, 256, 1, 1, 0, 7.9, 1.09, 1.61, 0}};
 
