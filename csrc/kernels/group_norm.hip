@@ -394,18 +394,21 @@ __global__ __launch_bounds__(NT) void apply(DmlGroupNormArgs a, int S, int rows,
   write(h, f, a.act, count, nullptr, y + s.rt * a.ldy, s.RT * a.ldy);
 }
 
-// What no slab fits: groups wider than 1024 vectors, fewer channels than a vector has. A workgroup per
-// (sample, group), element by element, three reads.
+// What no slab fits: fewer channels than a vector has, groups wider than 1024 vectors, and group counts without a
+// divisor up to kMaxGroups that makes a vector (521 groups of one channel). A workgroup per (sample, group), element by
+// element, three reads: bound by one CU's instructions and latency (1 x 2^22 x 3 in one group: 52 ms). A thread may
+// add 2^20 values and more one after the other, so the sums are in 64 bits (in 32, 2^25 x 3 fp16 values at a level of
+// 100 and a spread of 1 came out up to 3 times the rounding off).
 template <class T>
 __global__ __launch_bounds__(256) void by_element(DmlGroupNormArgs a) {
-  __shared__ float part[4];
+  __shared__ double part[4];
   const int g = blockIdx.x % a.G, n = blockIdx.x / a.G;
   const int cg = a.C / a.G, c0 = g * cg;
   const int64_t count = (int64_t)a.HW * cg;
   const T* x = (const T*)a.x + n * a.xn + c0;
   T* y = (T*)a.y + n * a.yn + c0;
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  auto total = [&](float v) {
+  auto total = [&](double v) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
     __syncthreads();
@@ -413,15 +416,15 @@ __global__ __launch_bounds__(256) void by_element(DmlGroupNormArgs a) {
     __syncthreads();
     return part[0] + part[1] + part[2] + part[3];
   };
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < count; i += 256) s += to_f32(x[(i / cg) * a.ldx + i % cg]);
-  const float mu = total(s) / (float)count;
-  s = 0.f;
+  double s = 0;
+  for (int64_t i = threadIdx.x; i < count; i += 256) s += (double)to_f32(x[(i / cg) * a.ldx + i % cg]);
+  const float mu = (float)(total(s) / (double)count);
+  s = 0;
   for (int64_t i = threadIdx.x; i < count; i += 256) {
     const float d = to_f32(x[(i / cg) * a.ldx + i % cg]) - mu;
-    s += d * d;
+    s += (double)(d * d);
   }
-  const float rs = inv_sqrt(total(s) / (float)count + a.eps);
+  const float rs = inv_sqrt((float)(total(s) / (double)count) + a.eps);
   for (int64_t i = threadIdx.x; i < count; i += 256) {
     const int c = (int)(i % cg);
     const float v = (to_f32(x[(i / cg) * a.ldx + c]) - mu) * (rs * (a.weight ? a.weight[c0 + c] : 1.f)) +
