@@ -550,13 +550,14 @@ static long row_tiles(const DmlProductArgs* a, int bm) {
   return (a->M + (used + a->fill) * (bm - 1)) / bm;
 }
 
+static long tiles_of(const DmlProductArgs* a, int bm, int bn) { return row_tiles(a, bm) * ((a->N + bn - 1) / bn); }
+
+// a grid has under 2^32 threads
+static bool launchable(long blocks, int threads) { return blocks <= (long)(UINT_MAX / threads); }
+
 template <class C>
 static int launch(const DmlProductArgs* a, hipStream_t s) {
-  const long blocks = row_tiles(a, C::BM) * ((a->N + C::BN - 1) / C::BN);
-  if (blocks > (long)(UINT_MAX / C::NT)) {
-    dml_set_error("dml_product: over 2^32 threads");
-    return -1;
-  }
+  const long blocks = tiles_of(a, C::BM, C::BN);
   hipLaunchKernelGGL(product_tile<C>, dim3((unsigned)blocks), dim3(C::NT), 0, s, *a);
   DML_CHECK_LAUNCH();
   return 0;
@@ -564,11 +565,7 @@ static int launch(const DmlProductArgs* a, hipStream_t s) {
 
 template <class T, int F, int NW, int U>
 static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
-  const long blocks = row_tiles(a, 16 * F) * ((a->N + 16 * F - 1) / (16 * F));
-  if (blocks > (long)(UINT_MAX / (NW * 64))) {
-    dml_set_error("dml_product: over 2^32 threads");
-    return -1;
-  }
+  const long blocks = tiles_of(a, 16 * F, 16 * F);
   hipLaunchKernelGGL((product_rows<T, F, F, NW, U>), dim3((unsigned)blocks), dim3(NW * 64), 0, s, *a);
   DML_CHECK_LAUNCH();
   return 0;
@@ -582,15 +579,13 @@ static int launch_rows(const DmlProductArgs* a, hipStream_t s) {
 // 64 with 4 (more workgroups to load); 1024 x 512 x 2048 7.6 with KG = 1, 8.6 with 2, 11.3 with 4; 17664 x 1024 x 4096 192
 // in tiles of 256, 160 of 192 x 128, 180 of 128; 16384 x 4096 x 4096 430 / 462 / 500; 6304 x 4096 x 1024 83 / 76 / 54.
 struct Form {
-  int bm, bn, kg, per_cu;
+  int bm, bn, kg, per_cu, threads;
   double first, fixed, low, high, shared;
 };
-constexpr Form kForms[] = {{32, 32, 8, 1, 1.8, 2.3, 0.50, 0.84, 0},     {64, 64, 1, 4, 2.7, 0.6, 0.21, 0.44, 0.18},
-                           {64, 64, 2, 2, 2.3, 1.4, 0.30, 0.69, 0},     {64, 64, 4, 1, 1.9, 2.7, 0.51, 0.99, 0},
-                           {128, 128, 1, 2, 2.5, 2.6, 0.41, 0.81, 0.42}, {192, 128, 1, 2, 2.8, 3.6, 0.57, 1.09, 0},
-                           {256, 256, 1, 1, 0, 7.9, 1.09, 1.61, 0}};
-
-static long tiles_of(const DmlProductArgs* a, int bm, int bn) { return row_tiles(a, bm) * ((a->N + bn - 1) / bn); }
+constexpr Form kForms[] = {{32, 32, 8, 1, 512, 1.8, 2.3, 0.50, 0.84, 0},     {64, 64, 1, 4, 256, 2.7, 0.6, 0.21, 0.44, 0.18},
+                           {64, 64, 2, 2, 512, 2.3, 1.4, 0.30, 0.69, 0},     {64, 64, 4, 1, 1024, 1.9, 2.7, 0.51, 0.99, 0},
+                           {128, 128, 1, 2, 256, 2.5, 2.6, 0.41, 0.81, 0.42}, {192, 128, 1, 2, 256, 2.8, 3.6, 0.57, 1.09, 0},
+                           {256, 256, 1, 1, 512, 0, 7.9, 1.09, 1.61, 0}};
 
 static double cost(const DmlProductArgs* a, const Form& f, bool dma) {
   const long tiles = tiles_of(a, f.bm, f.bn), per = (tiles + 255) / 256, rounds = per / f.per_cu, rest = per % f.per_cu;
@@ -617,14 +612,19 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
   const double rows16 = 3.1 + (tiles_of(a, 16, 16) + 255) / 256 * (k < 0.45 ? 0.45 : k) * (a->M <= 16 ? 3.0 : 3.6);
   const double each32 = 1.3 + 0.3 * (t32 < 256 ? t32 / 256 : 1.0), all32 = ((long)t32 + 255) / 256 * ((a->K + 511) / 512) * each32;
   const double rows32 = dma ? 3.1 + all32 : 3.8 + 1.25 * all32;
-  double least = rows16 < rows32 ? rows16 : rows32;
-  int best = rows16 < rows32 ? -1 : -2;
+  // the cheapest that a grid holds: products of 2^30 rows take larger tiles
+  int best = -3;
+  double least = 1e300;
+  if (launchable(tiles_of(a, 16, 16), 16 * 64)) least = rows16, best = -1;
+  if (launchable((long)t32, 8 * 64) && rows32 <= least) least = rows32, best = -2;
   for (int i = 0; i < (int)(sizeof(kForms) / sizeof(kForms[0])); ++i) {
     if (!dma && (kForms[i].bm > 128 || kForms[i].kg == 2 || kForms[i].kg == 8)) continue;  // not built through registers
+    if (!launchable(tiles_of(a, kForms[i].bm, kForms[i].bn), kForms[i].threads)) continue;
     const double c = cost(a, kForms[i], dma);
     if (c < least) least = c, best = i;
   }
   switch (best) {
+    case -3: dml_set_error("dml_product: over 2^32 threads"); return -1;
     case -2: return launch_rows<T, 2, 8, 1>(a, s);
     case -1: return launch_rows<T, 1, 16, 2>(a, s);
     case 0: return launch<Tile<T, 32, 32, 1, 1, 8, true>>(a, s);

@@ -137,3 +137,13 @@ def test_products_into_their_residual(m, k, n, out_dtype):
         ops.linear(x, w, b, residual=y, out=y, **kw)
         ops.grouped_linear(x, pair, ends, residual=z, act_last=True, out=z, **kw)
         assert torch.equal(y, want[0]) and torch.equal(z, want[1])
+
+
+def test_linear_of_more_than_2_30_rows():
+    """More rows than 2^32 threads hold in tiles of 64."""
+    row = torch.tensor([1.0, -2.0, 3.0, 0.0, 0.5, 0.0, 0.0, 4.0], device="cuda", dtype=BF)
+    m = 2 ** 30 + 77
+    y = ops.linear(row.expand(m, 8), torch.ones(1, 8, device="cuda", dtype=BF))
+    assert y.shape == (m, 1)
+    for part in y.split(2 ** 28):
+        assert (part == 6.5).all()
