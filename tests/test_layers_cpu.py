@@ -253,3 +253,31 @@ def test_forward_mode_tangents_are_refused(call, no_grad):
 def test_forward_mode_through_a_function_transform():
     with pytest.raises(ValueError, match="no derivative"):
         torch.func.jvp(lambda t: _norm(t), (_t(2, 3, 3, 16),), (_t(2, 3, 3, 16),))
+
+
+def _merged(x, groups, rows, between=True, lost=None, last_full=False):
+    """Group norm from chunks of `rows` positions, merged in fp32, or with a mistake in the merge."""
+    n, c = x.shape[0], x.shape[-1]
+    v = x.float().reshape(n, -1, groups, c // groups)
+    chunks = [p for i, p in enumerate(v.split(rows, 1)) if i != lost]
+    mean = torch.stack([p.mean((1, 3)) for p in chunks])
+    m2 = torch.stack([(p - p.mean((1, 3), keepdim=True)).square().sum((1, 3)) for p in chunks])
+    size = torch.tensor([rows if last_full else p.shape[1] for p in chunks]).float()[:, None, None] * (c // groups)
+    mu = (mean * size).sum(0) / size.sum()
+    var = (m2 + (size * (mean - mu).square() if between else 0)).sum(0) / size.sum()
+    return ((v - mu[:, None, :, None]) / torch.sqrt(var + 1e-5)[:, None, :, None]).reshape(x.shape).to(x.dtype)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+@pytest.mark.parametrize("drift", ("ramp", "steps"))
+def test_the_tolerance_of_merged_chunks_tells_mistakes(drift, dtype):
+    """The bound that the kernels' merged chunks are held to accepts a right merge, and no missing term or chunk."""
+    from test_layers_edges_gpu import drifting, steps_of_chunks, tight64
+    from test_layers_gpu import close
+
+    x = (torch.randn(1, 9000, 48, generator=torch.Generator().manual_seed(3)) + drifting(drift, 9000, "cpu")).to(dtype)
+    y, err = tight64(x, 3, steps_of_chunks())
+    close(_merged(x, 3, 512), y, err)
+    for mistake in ({"between": False}, {"lost": 7}, {"lost": 17}, {"last_full": True}):
+        with pytest.raises(AssertionError, match="times the tolerance"):
+            close(_merged(x, 3, 512, **mistake), y, err)

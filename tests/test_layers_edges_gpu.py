@@ -90,6 +90,15 @@ def test_group_norm_of_groups_beyond_31_bits(positions, c):
     torch.cuda.empty_cache()
 
 
+def steps_of_chunks():
+    """Additions in a row, at most, on the way from a value to its group's mean or sum of squares where a sample goes
+    through chunks: a thread's own (8 rows, as many values each as a vector has where that is one statistic: 64), the
+    workgroup's merge (with a statistic per vector NT / 64 = 16 a lane, with one per channel 8 times that, but then a
+    thread has 8 values: so 8 + 128), 6 levels over lanes; then, by 8 lanes, fewer than 2048 chunks, or with `join` far
+    fewer: 256 + 6; a dozen for the products, the division and the last subtraction."""
+    return 8 + 128 + 6 + 256 + 6 + 12
+
+
 def tight64(x, groups, d, eps=1e-5):
     """(y, err) of the norm without its affine map: fp32 statistics over chains of d operations, centred and merged.
 
@@ -105,6 +114,25 @@ def tight64(x, groups, d, eps=1e-5):
     rs = 1 / torch.sqrt(var + eps)
     y = (xd - mu) * rs
     return y.reshape(x.shape), ((e + u * (xd - mu).abs()) * rs * (1 + rel) + y.abs() * (rel + 4 * u)).reshape(x.shape)
+
+
+def drifting(drift, positions, device):
+    """Levels along a sample, [positions, 1]."""
+    p = torch.arange(positions, device=device) / positions
+    return {"ramp": 16 * p - 8, "steps": 10 * (p * 7).floor().remainder(3) - 10, "level": 50 + 0 * p}[drift][:, None]
+
+
+@pytest.mark.parametrize("drift", ("ramp", "steps", "level"))
+@pytest.mark.parametrize("dtype", (BF, FP))
+@pytest.mark.parametrize("shape, groups", [((1, 9000, 96), 3), ((1, 20000, 64), 8), ((2, 70001, 256), 32), ((1, 300000, 64), 8),
+                                           ((1, 400000, 35), 5), ((1, 150000, 520), 520), ((1, 30011, 99), 9)])
+def test_group_norm_merges_chunks_of_different_levels(shape, groups, dtype, drift):
+    """The levels drift along the sample, so that the distances between the chunks' means are most of the variance."""
+    g = gen(31)
+    x = (normal(g, *shape) + drifting(drift, shape[1], "cuda")).to(dtype)
+    y, err = tight64(x, groups, steps_of_chunks())
+    assert err.max() < 0.02  # a lost chunk or a missing term between them is far more
+    close(ops.group_norm(x, groups), y, err)
 
 
 @pytest.mark.parametrize("dtype", (BF, HF, FP))
