@@ -607,7 +607,9 @@ static int dispatch(const DmlProductArgs* a, hipStream_t s) {
                    255 * (a->ldx > a->ldw ? a->ldx : a->ldw) + a->K < (1 << 30) - 512 && a->K < (1 << 22);
   // product_rows in 16 x 16 (16 waves: 2048 of K in flight) and 32 x 32 (8 waves, 512), by the same timings: a workgroup
   // on a CU takes 3.6 us per 2048 of K, less where there is one tile of rows, and 1.3 to 1.6 per 512 (more
-  // off the dword grid: 67 x 519 x 1388 takes 6.8 us in 16 x 16, 7.9 in 32 x 32)
+  // off the dword grid: 67 x 519 x 1388 takes 6.8 us in 16 x 16, 7.9 in 32 x 32). Off the 16-byte grid the choice among
+  // these and the forms through registers was 3.1 % slower than the best in the mean over 130 products, 34 % at worst
+  // (591 x 152 x 598).
   const double k = a->K / 2048.0, t32 = (double)tiles_of(a, 32, 32);
   const double rows16 = 3.1 + (tiles_of(a, 16, 16) + 255) / 256 * (k < 0.45 ? 0.45 : k) * (a->M <= 16 ? 3.0 : 3.6);
   const double each32 = 1.3 + 0.3 * (t32 < 256 ? t32 / 256 : 1.0), all32 = ((long)t32 + 255) / 256 * ((a->K + 511) / 512) * each32;

@@ -2,7 +2,8 @@
 
 Channels last like every op here: the last dimension is contiguous, the leading ones may be a slice of a
 wider (concat) buffer. Forward only, on the tensors' device and its current stream; a call allocates its
-output and nothing that outlives it, so it can be captured into a graph. Wrong arguments raise TypeError
+output and nothing that outlives it, so it can be captured into a graph. Weight and bias of a norm and bias of a
+product are read in fp32: in x's type, each costs a conversion per call. Wrong arguments raise TypeError
 or ValueError before anything is launched, a failure of the library raises ``NativeError``.
 """
 from __future__ import annotations
