@@ -15,6 +15,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 
@@ -178,6 +179,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     device = _ready(x, weight, bias, out)
     if out is None:
         out = x.new_empty(shape)
+    else:
+        increment_version(out)  # a backward pass that saved out's old values refuses instead of reading the new ones
     if not (n and rows):
         return out
     weight, bias = _f32(weight), _f32(bias)
@@ -236,6 +239,8 @@ def _product(x, weight, ends, bias, act, residual, act_last, out, out_dtype, wha
     if out is None:
         out = x.new_empty(shape, dtype=to)
         fill = int(ends is not None)
+    else:
+        increment_version(out)  # as in group_norm
     if not (m and n):
         return out
     if e == 0:

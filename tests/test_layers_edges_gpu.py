@@ -175,3 +175,21 @@ def test_linear_of_more_than_2_30_rows():
     assert y.shape == (m, 1)
     for part in y.split(2 ** 28):
         assert (part == 6.5).all()
+
+
+def test_out_that_a_backward_pass_saved():
+    """Writing into a tensor that some graph saved is seen by autograd, as with any in-place operation."""
+    g = gen(41)
+    x, w = normal(g, 8, 16).to(BF), normal(g, 16, 16).to(BF)
+    ends = torch.tensor([3, 8], device="cuda")
+    for call in (lambda t: ops.group_norm(x, 4, out=t), lambda t: ops.linear(x, w, out=t),
+                 lambda t: ops.linear(x, w, residual=t, out=t), lambda t: ops.grouped_linear(x, torch.stack([w, w]), ends, out=t)):
+        leaf, saved = torch.ones(8, 16, device="cuda", dtype=BF, requires_grad=True), normal(g, 8, 16).to(BF)
+        y = (leaf * saved).sum()
+        with torch.no_grad():
+            call(saved)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    with torch.inference_mode():
+        out = torch.empty(8, 16, device="cuda", dtype=BF)
+        assert torch.equal(ops.linear(x, w, out=out), ops.linear(x, w))
